@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIBGSX = os.path.join(HERE, "libgsx.so")
-HIP_SOURCES = ["gsx_capi.hip", "gsx_sh.hip", "gsx_projection.hip", "gsx_intersect.hip", "gsx_raster.hip", "gsx_raster_fast.hip", "gsx_frontend.hip", "gsx_mcmc.hip", "gsx_adam.hip", "gsx_ssim.hip"]
+HIP_SOURCES = ["gsx_capi.hip", "gsx_sh.hip", "gsx_projection.hip", "gsx_intersect.hip", "gsx_raster.hip", "gsx_raster_fast.hip", "gsx_frontend.hip", "gsx_mcmc.hip", "gsx_adam.hip", "gsx_adamw.hip", "gsx_ssim.hip"]
 HIP_HEADERS = ["gsx_device.hpp", "gsx_raster_common.hpp", "gsx_record.hpp", "gsx_sh_basis.hpp", "gsx_ut_project.hpp"]
 
 
@@ -52,7 +52,7 @@ def _run(cmd):
 
 def build_libgsx(force=False, verbose=False):
     srcs = [os.path.join(CSRC, s) for s in HIP_SOURCES]
-    deps = srcs + [os.path.join(CSRC, h) for h in HIP_HEADERS] + [os.path.join(INCLUDE, "gsx.h")]
+    deps = srcs + [os.path.join(CSRC, h) for h in HIP_HEADERS] + [os.path.join(INCLUDE, "gsx.h"), os.path.join(INCLUDE, "gsx_optim.h")]
     if not (force or _newer(LIBGSX, deps)):
         return LIBGSX
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -85,7 +85,7 @@ BACKEND = os.path.join(HERE, "libgsx_gsplat_backend.so")
 
 def _shim_deps():
     src = os.path.join(CSRC, "ops_shim.cpp")
-    return src, [src, os.path.join(INCLUDE, "gsx.h"), os.path.join(INCLUDE, "gsx_ops.h"), os.path.join(INCLUDE, "gsx_training_ops.h")] + \
+    return src, [src, os.path.join(INCLUDE, "gsx.h"), os.path.join(INCLUDE, "gsx_ops.h"), os.path.join(INCLUDE, "gsx_training_ops.h"), os.path.join(INCLUDE, "gsx_optim.h")] + \
         [os.path.join(COMPAT, h) for h in ("Ops.h", "Cameras.h", "Common.h", "Projection.h")]
 
 

@@ -15,10 +15,12 @@
 
 #include <ATen/hip/HIPEvent.h>
 
+#include <algorithm>
 #include <atomic>
 #include <chrono>
 #include <cstdlib>
 #include <cstring>
+#include <limits>
 #include <map>
 #include <mutex>
 #include <string>
@@ -27,6 +29,7 @@
 
 #include "../../include/gsx.h"
 #include "../../include/gsx_ops.h"
+#include "../../include/gsx_optim.h"
 #include "../../include/gsx_training_ops.h"
 
 namespace {
@@ -45,6 +48,8 @@ namespace {
 const bool abi_checked = [] {
     TORCH_CHECK(gsx_abi_version() == GSX_ABI_VERSION, "libgsx.so has ABI version ", gsx_abi_version(), ", this shim was built against ", GSX_ABI_VERSION,
                 " (include/gsx.h): rebuild both");
+    TORCH_CHECK(gsx_optim_abi_version() == GSX_OPTIM_ABI_VERSION, "libgsx.so has optimizer ABI version ", gsx_optim_abi_version(),
+                ", this shim was built against ", GSX_OPTIM_ABI_VERSION, " (include/gsx_optim.h): rebuild both");
     return true;
 }();
 
@@ -1183,6 +1188,190 @@ void adam_step(at::Tensor param, at::Tensor exp_avg, at::Tensor exp_avg_sq, cons
                         (float)bias_correction2_sqrt_rcp, cur_stream()), "adam_step");
 }
 
+// ---- the optimizer operators over many tensors (include/gsx_optim.h) -------------------------------------------------------------------------------
+namespace {
+
+uint32_t optim_dtype(const at::Tensor& t, const char* op, const char* what, size_t i) {
+    if (t.scalar_type() == at::kFloat) return GSX_DTYPE_F32;
+    if (t.scalar_type() == at::kBFloat16) return GSX_DTYPE_BF16;
+    TORCH_CHECK(t.scalar_type() == at::kHalf, op, ": ", what, " ", i, " is ", t.scalar_type(), "; float32, bfloat16 or float16 are supported");
+    return GSX_DTYPE_F16;
+}
+
+// [rows, cols] with rows ld apart: dense tensors, and views of the leading dimension's rows whose values lie next to each other (sh[:, 1:]).
+void rows_of(const at::Tensor& t, uint64_t& rows, uint64_t& cols, uint64_t& ld, const char* op, const char* what, size_t i) {
+    const uint64_t n = (uint64_t)t.numel();
+    if (n == 0 || t.is_contiguous()) { rows = 1; cols = ld = n; return; }
+    int64_t inner = 1;
+    for (int64_t d = t.dim() - 1; d >= 1; --d) {
+        TORCH_CHECK(t.size(d) == 1 || t.stride(d) == inner, op, ": ", what, " ", i, " is neither dense nor a row-strided view (sizes ", t.sizes(), ", strides ",
+                    t.strides(), "): make it contiguous");
+        inner *= t.size(d);
+    }
+    rows = (uint64_t)t.size(0); cols = (uint64_t)inner; ld = (uint64_t)t.stride(0);
+    TORCH_CHECK(t.stride(0) >= inner, op, ": ", what, " ", i, " has rows that overlap (sizes ", t.sizes(), ", strides ", t.strides(), "): make it contiguous");
+}
+
+void check_on(const at::Tensor& t, const at::Device& dev, const char* op, const char* what, size_t i) {
+    TORCH_CHECK(t.is_cuda() && t.device() == dev, op, ": ", what, " ", i, " is on ", t.device(), ", the first tensor on ", dev);
+}
+
+const double* control_of(const at::optional<at::Tensor>& control, const at::Device& dev, const char* op) {
+    if (!control.has_value() || !control->defined()) return nullptr;
+    TORCH_CHECK(control->scalar_type() == at::kDouble && control->is_contiguous() && control->numel() == GSX_CONTROL_WORDS, op,
+                ": the control block is a float64 tensor of ", GSX_CONTROL_WORDS, " values (ops.step_control)");
+    check_on(*control, dev, op, "the control block", 0);
+    return control->data_ptr<double>();
+}
+
+using Splits = std::vector<std::tuple<int64_t, double, double, bool, bool>>;
+
+// What both AdamW operators share; `scales` is empty for moments in 32 bits.
+void adamw_multi(const char* op, const std::vector<at::Tensor>& params, const std::vector<at::Tensor>& exp_avgs, const std::vector<at::Tensor>& exp_avg_sqs,
+                 const std::vector<at::Tensor>& avg_scales, const std::vector<at::Tensor>& rms_scales, bool eight, const std::vector<at::Tensor>& grads,
+                 const std::vector<double>& lrs, const std::vector<double>& weight_decays, double beta1, double beta2, double eps,
+                 const std::vector<int64_t>& steps, const at::optional<at::Tensor>& control, const Splits& splits, const at::optional<int64_t>& seed) {
+    const size_t k = params.size();
+    TORCH_CHECK(exp_avgs.size() == k && exp_avg_sqs.size() == k && grads.size() == k && lrs.size() == k && weight_decays.size() == k &&
+                (steps.empty() || steps.size() == k) && (splits.empty() || splits.size() == k) && (!eight || (avg_scales.size() == k && rms_scales.size() == k)),
+                op, ": the lists have one entry for each of the ", k, " parameters (steps and splits may be empty)");
+    TORCH_CHECK(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, op, ": betas lie in [0, 1), got ", beta1, ", ", beta2);
+    TORCH_CHECK(eps >= 0, op, ": eps is not negative, got ", eps);
+    if (k == 0) return;
+    GSX_DEVICE_GUARD(params[0]);
+    const at::Device dev = params[0].device();
+    const double* ctl = control_of(control, dev, op);
+    TORCH_CHECK(!steps.empty() || ctl != nullptr, op, ": steps may be empty only with a control block");
+    TORCH_CHECK(!seed.has_value() || (*seed >= 0 && *seed <= 0xFFFFFFFFll), op, ": seed lies in 0 .. 2^32 - 1");
+    std::vector<gsx_adamw_tensor> list(k);
+    std::vector<const void*> written;
+    for (size_t i = 0; i < k; ++i) {
+        const at::Tensor &p = params[i], &g = grads[i], &m = exp_avgs[i], &v = exp_avg_sqs[i];
+        check_on(p, dev, op, "parameter", i); check_on(g, dev, op, "gradient", i); check_on(m, dev, op, "exp_avg", i); check_on(v, dev, op, "exp_avg_sq", i);
+        TORCH_CHECK(p.sizes() == g.sizes(), op, ": parameter ", i, " has sizes ", p.sizes(), ", its gradient ", g.sizes());
+        TORCH_CHECK(m.numel() == p.numel() && v.numel() == p.numel(), op, ": the moments of parameter ", i, " have ", m.numel(), " and ", v.numel(), " values, not ", p.numel());
+        const auto state = eight ? at::kFloat8_e4m3fn : at::kFloat;
+        TORCH_CHECK(m.scalar_type() == state && v.scalar_type() == state && m.is_contiguous() && v.is_contiguous(), op, ": the moments of parameter ", i,
+                    " are contiguous ", state, " tensors");
+        gsx_adamw_tensor& x = list[i];
+        x = gsx_adamw_tensor{};
+        x.param_dtype = optim_dtype(p, op, "parameter", i);
+        x.grad_dtype = optim_dtype(g, op, "gradient", i);
+        uint64_t rp, cp, rg, cg;
+        rows_of(p, rp, cp, x.ld_param, op, "parameter", i);
+        rows_of(g, rg, cg, x.ld_grad, op, "gradient", i);
+        const auto split = splits.empty() ? std::make_tuple((int64_t)0, 0.0, 0.0, false, false) : splits[i];
+        // a dense tensor counts as one row unless something goes by rows: the other of the two, or the column groups
+        x.rows = rp; x.cols = cp;
+        const bool groups = std::get<0>(split) != 0;
+        if (p.numel() != 0 && (rp != rg || cp != cg || groups)) {
+            TORCH_CHECK(p.dim() >= 1, op, ": a split needs rows");
+            x.rows = (uint64_t)p.size(0); x.cols = (uint64_t)(p.numel() / p.size(0));
+            if (rp == 1 && cp == (uint64_t)p.numel()) x.ld_param = x.cols;
+            if (rg == 1 && cg == (uint64_t)g.numel()) x.ld_grad = x.cols;
+        }
+        if (groups)
+            TORCH_CHECK(std::get<0>(split) > 0 && (p.numel() == 0 || (uint64_t)std::get<0>(split) <= x.cols), op, ": split ", std::get<0>(split), " of parameter ", i,
+                        " lies beyond its ", x.cols, " columns");
+        x.param = p.data_ptr(); x.grad = g.data_ptr(); x.exp_avg = m.data_ptr(); x.exp_avg_sq = v.data_ptr();
+        if (eight) {
+            const int64_t runs = (p.numel() + GSX_MOMENT_RUN - 1) / GSX_MOMENT_RUN;
+            for (const at::Tensor* s : {&avg_scales[i], &rms_scales[i]}) {
+                check_on(*s, dev, op, "scale", i);
+                TORCH_CHECK(s->scalar_type() == at::kFloat && s->is_contiguous() && s->numel() == runs, op, ": the scales of parameter ", i, " are contiguous float32 tensors of ",
+                            runs, " values, one for each ", GSX_MOMENT_RUN);
+            }
+            x.avg_scale = avg_scales[i].data_ptr<float>(); x.rms_scale = rms_scales[i].data_ptr<float>();
+        }
+        x.split = (uint32_t)std::get<0>(split); x.lr_b = (float)std::get<1>(split); x.weight_decay_b = (float)std::get<2>(split);
+        x.hold = std::get<3>(split); x.hold_b = std::get<4>(split);
+        x.lr = (float)lrs[i]; x.weight_decay = (float)weight_decays[i];
+        if (!steps.empty()) {
+            TORCH_CHECK(steps[i] >= 1 && steps[i] <= 0xFFFFFFFFll, op, ": steps count from 1, got ", steps[i], " for parameter ", i);
+            x.step = (uint64_t)steps[i];
+        }
+        if (p.numel() != 0) written.push_back(x.param);
+    }
+    std::sort(written.begin(), written.end());
+    TORCH_CHECK(std::adjacent_find(written.begin(), written.end()) == written.end(), op, ": a parameter is in the list twice");
+    if (eight) check(gsx_adamw8_step_multi((uint32_t)k, list.data(), beta1, beta2, eps, seed.has_value(), (uint32_t)seed.value_or(0), ctl, cur_stream()), op);
+    else check(gsx_adamw_step_multi((uint32_t)k, list.data(), beta1, beta2, eps, ctl, cur_stream()), op);
+}
+
+}  // namespace
+
+void adamw_step_multi(std::vector<at::Tensor> params, std::vector<at::Tensor> exp_avgs, std::vector<at::Tensor> exp_avg_sqs, std::vector<at::Tensor> grads,
+                      std::vector<double> lrs, std::vector<double> weight_decays, double beta1, double beta2, double eps, std::vector<int64_t> steps,
+                      at::optional<at::Tensor> control, Splits splits) {
+    adamw_multi("adamw_step_multi", params, exp_avgs, exp_avg_sqs, {}, {}, false, grads, lrs, weight_decays, beta1, beta2, eps, steps, control, splits, at::nullopt);
+}
+
+void adamw8_step_multi(std::vector<at::Tensor> params, std::vector<at::Tensor> exp_avgs, std::vector<at::Tensor> exp_rmss, std::vector<at::Tensor> avg_scales,
+                       std::vector<at::Tensor> rms_scales, std::vector<at::Tensor> grads, std::vector<double> lrs, std::vector<double> weight_decays,
+                       double beta1, double beta2, double eps, std::vector<int64_t> steps, at::optional<at::Tensor> control, Splits splits,
+                       at::optional<int64_t> seed) {
+    adamw_multi("adamw8_step_multi", params, exp_avgs, exp_rmss, avg_scales, rms_scales, true, grads, lrs, weight_decays, beta1, beta2, eps, steps, control, splits, seed);
+}
+
+void grad_norm_multi(std::vector<at::Tensor> grads, at::Tensor control, double max_norm) {
+    const char* op = "grad_norm_multi";
+    GSX_DEVICE_GUARD(control);
+    const at::Device dev = control.device();
+    double* ctl = const_cast<double*>(control_of(control, dev, op));
+    TORCH_CHECK(ctl != nullptr, op, ": a control block is needed");
+    TORCH_CHECK(max_norm > 0, op, ": max_norm is positive (infinite for no clipping), got ", max_norm);
+    std::vector<gsx_grad_tensor> list(grads.size());
+    for (size_t i = 0; i < grads.size(); ++i) {
+        check_on(grads[i], dev, op, "gradient", i);
+        gsx_grad_tensor& x = list[i];
+        x.dtype = optim_dtype(grads[i], op, "gradient", i);
+        rows_of(grads[i], x.rows, x.cols, x.ld, op, "gradient", i);
+        x.grad = grads[i].data_ptr();
+    }
+    const size_t bytes = gsx_grad_norm_multi_workspace_bytes((uint32_t)list.size(), list.data());
+    at::Tensor ws = at::empty({(int64_t)bytes}, control.options().dtype(at::kByte));
+    check(gsx_grad_norm_multi((uint32_t)list.size(), list.data(), max_norm, ctl, ws.data_ptr(), bytes, cur_stream()), op);
+}
+
+std::tuple<std::vector<at::Tensor>, std::vector<at::Tensor>, std::vector<at::Tensor>, std::vector<at::Tensor>>
+adamw8_select_rows(std::vector<at::Tensor> exp_avgs, std::vector<at::Tensor> exp_rmss, std::vector<at::Tensor> avg_scales, std::vector<at::Tensor> rms_scales,
+                   at::Tensor index) {
+    const char* op = "adamw8_select_rows";
+    const size_t k = exp_avgs.size();
+    TORCH_CHECK(exp_rmss.size() == k && avg_scales.size() == k && rms_scales.size() == k, op, ": four lists of equal length");
+    GSX_DEVICE_GUARD(index);
+    const at::Device dev = index.device();
+    TORCH_CHECK(index.scalar_type() == at::kLong && index.dim() == 1 && index.is_contiguous(), op, ": index is a contiguous int64 vector");
+    const int64_t rows_out = index.numel();
+    const int64_t rows_in = k ? (exp_avgs[0].dim() ? exp_avgs[0].size(0) : 0) : 0;
+    std::vector<at::Tensor> out[4];
+    std::vector<gsx_moments8> list(k);
+    for (size_t i = 0; i < k; ++i) {
+        const at::Tensor *in[4] = {&exp_avgs[i], &exp_rmss[i], &avg_scales[i], &rms_scales[i]};
+        for (int j = 0; j < 2; ++j) {
+            check_on(*in[j], dev, op, "moments", i);
+            TORCH_CHECK(in[j]->scalar_type() == at::kFloat8_e4m3fn && in[j]->is_contiguous() && in[j]->dim() >= 1 && in[j]->size(0) == rows_in &&
+                        in[j]->sizes() == exp_avgs[i].sizes(), op, ": the moments ", i, " are contiguous float8_e4m3fn tensors of ", rows_in, " rows");
+        }
+        int64_t cols = 1;
+        for (int64_t d = 1; d < exp_avgs[i].dim(); ++d) cols *= exp_avgs[i].size(d);
+        for (int j = 2; j < 4; ++j) {
+            check_on(*in[j], dev, op, "scales", i);
+            TORCH_CHECK(in[j]->scalar_type() == at::kFloat && in[j]->is_contiguous() && in[j]->numel() == (rows_in * cols + GSX_MOMENT_RUN - 1) / GSX_MOMENT_RUN, op,
+                        ": the scales ", i, " are contiguous float32 tensors with one value for each ", GSX_MOMENT_RUN);
+        }
+        auto sizes = exp_avgs[i].sizes().vec();
+        sizes[0] = rows_out;
+        const int64_t runs = (rows_out * cols + GSX_MOMENT_RUN - 1) / GSX_MOMENT_RUN;
+        for (int j = 0; j < 2; ++j) out[j].push_back(at::empty(sizes, in[j]->options()));
+        for (int j = 2; j < 4; ++j) out[j].push_back(at::empty({runs}, in[j]->options()));
+        list[i] = gsx_moments8{in[0]->data_ptr(), in[1]->data_ptr(), in[2]->data_ptr<float>(), in[3]->data_ptr<float>(), out[0][i].data_ptr(), out[1][i].data_ptr(),
+                               out[2][i].data_ptr<float>(), out[3][i].data_ptr<float>(), (uint64_t)cols};
+    }
+    check(gsx_adamw8_select_rows((uint32_t)k, list.data(), (uint64_t)rows_in, (uint64_t)rows_out, index.data_ptr<int64_t>(), cur_stream()), op);
+    return std::make_tuple(out[0], out[1], out[2], out[3]);
+}
+
 }  // namespace gsx_ext
 
 // ---------------------------------------------------------------------------------------------
@@ -1388,6 +1577,17 @@ PYBIND11_MODULE(_gsx_ops, m) {
     });
     m.def("adam_step", &gsx_ext::adam_step);
     m.def("adam_step_multi", &gsx_ext::adam_step_multi);
+    m.attr("MOMENT_RUN") = GSX_MOMENT_RUN;
+    m.attr("CONTROL_WORDS") = GSX_CONTROL_WORDS;
+    m.def("adamw_step_multi", &gsx_ext::adamw_step_multi, py::arg("params"), py::arg("exp_avgs"), py::arg("exp_avg_sqs"), py::arg("grads"), py::arg("lrs"),
+          py::arg("weight_decays"), py::arg("beta1"), py::arg("beta2"), py::arg("eps"), py::arg("steps"), py::arg("control") = py::none(),
+          py::arg("splits") = gsx_ext::Splits());
+    m.def("adamw8_step_multi", &gsx_ext::adamw8_step_multi, py::arg("params"), py::arg("exp_avgs"), py::arg("exp_rmss"), py::arg("avg_scales"),
+          py::arg("rms_scales"), py::arg("grads"), py::arg("lrs"), py::arg("weight_decays"), py::arg("beta1"), py::arg("beta2"), py::arg("eps"),
+          py::arg("steps"), py::arg("control") = py::none(), py::arg("splits") = gsx_ext::Splits(), py::arg("seed") = py::none());
+    m.def("grad_norm_multi", &gsx_ext::grad_norm_multi, py::arg("grads"), py::arg("control"), py::arg("max_norm") = std::numeric_limits<double>::infinity());
+    m.def("adamw8_select_rows", &gsx_ext::adamw8_select_rows, py::arg("exp_avgs"), py::arg("exp_rmss"), py::arg("avg_scales"), py::arg("rms_scales"),
+          py::arg("index"));
     m.def("adam_step_wrapper", [](at::Tensor param, at::Tensor exp_avg, at::Tensor exp_avg_sq, const at::Tensor grad, float lr, float beta1, float beta2,
                                   float eps, float bc1_rcp, float bc2_sqrt_rcp) {  // the reference's signature (adam_api.h:11-21)
         fast_gs::optimizer::adam_step_wrapper(param, exp_avg, exp_avg_sq, grad, lr, beta1, beta2, eps, bc1_rcp, bc2_sqrt_rcp);

@@ -65,6 +65,50 @@ splat_activations_bwd = _C.splat_activations_bwd
 adam_step = _C.adam_step
 adam_step_multi = _C.adam_step_multi
 adam_step_wrapper = _C.adam_step_wrapper
+
+
+# The optimizer operators over many tensors (include/gsx_optim.h).  Any number of tensors in a list, empty ones included; float32, bfloat16 or float16
+# parameters and gradients, dense or row-strided views (sh[:, 1:]); everything on one device, on its current stream; nothing waits for the device, all of them
+# may be captured into a graph (the numbers of the call are captured with it; step, clip factor and skip flag come from the control block).
+MOMENT_RUN = _C.MOMENT_RUN   # consecutive values of a tensor that share a scale of the 8-bit moments
+
+
+def step_control(device, step=0):
+    """The block through which grad_norm_multi steers the updates behind it without the host: float64 [norm, factor, skip, step, 4 internal words].  One block for
+    each sequence of calls (two streams, or two graphs in flight at once, take one each)."""
+    c = torch.zeros(_C.CONTROL_WORDS, dtype=torch.float64, device=device)
+    c[1], c[3] = 1.0, float(step)
+    return c
+
+
+def grad_norm_multi(grads, control, max_norm=float("inf")):
+    """control[0] = the norm of all gradients (accumulated in 64 bits, the same bits every time), [1] = min(1, max_norm / (norm + 1e-6)), [2] = 1 if a gradient
+    is infinite or NaN (the updates that read the block then leave everything as it is), [3] (the step) advanced by one if none is."""
+    _C.grad_norm_multi(grads, control, max_norm)
+
+
+def adamw_step_multi(params, exp_avgs, exp_avg_sqs, grads, lrs, weight_decays, beta1, beta2, eps, steps, control=None, splits=()):
+    """AdamW with decoupled decay on every tensor of the lists, in place: moments contiguous float32, a rate and a decay for each tensor.
+    steps: the number of this step for each tensor, from 1; empty: the control block's.  control (step_control): the gradients are multiplied by its factor,
+    and nothing is changed where its skip flag is set.  splits, one for each tensor or empty: (split, lr_b, weight_decay_b, hold_a, hold_b) — the columns
+    [split, ...) of a tensor seen as rows are a second group with its own rate and decay (0: one group); a held group and its moments stay as they are."""
+    _C.adamw_step_multi(params, exp_avgs, exp_avg_sqs, grads, lrs, weight_decays, beta1, beta2, eps, steps, control, splits)
+
+
+def adamw8_step_multi(params, exp_avgs, exp_rmss, avg_scales, rms_scales, grads, lrs, weight_decays, beta1, beta2, eps, steps, control=None, splits=(), seed=None):
+    """adamw_step_multi with the first moment and the root of the second as float8_e4m3fn tensors, each with one float32 scale for MOMENT_RUN consecutive values
+    (float32 [ceil(numel / MOMENT_RUN)]; zeros are zero moments).  seed None: rounded to nearest; 0 .. 2^32 - 1: stochastically, another draw for
+    every step, tensor of the list and value.  With rounding to nearest a moment that changes by less than half a step of the format (3 to 6 %) does not
+    change at all, and the second moment's average over 1 / (1 - beta2) steps comes to rest: training takes a seed."""
+    _C.adamw8_step_multi(params, exp_avgs, exp_rmss, avg_scales, rms_scales, grads, lrs, weight_decays, beta1, beta2, eps, steps, control, splits, seed)
+
+
+def adamw8_select_rows(exp_avgs, exp_rmss, avg_scales, rms_scales, index):
+    """Rows of 8-bit moments (permuted, removed, repeated, added) as new tensors: row j is row index[j] of the old ones, zero where index[j] is outside them.
+    All tensors have the same number of rows.  Returns the four lists."""
+    return _C.adamw8_select_rows(exp_avgs, exp_rmss, avg_scales, rms_scales, index)
+
+
 intersect_tile_binned = _C.intersect_tile_binned
 intersect_tile_binned_guarded = _C.intersect_tile_binned_guarded   # no host read of n_isects: (tiles_per_gauss, flatten_ids [capacity], offsets, IsectLists)
 shim_guarded_stats = _C.shim_guarded_stats
