@@ -1,0 +1,187 @@
+// gsx_adamw.hpp — what the optimizer operators over many tensors (include/gsx_optim.h) share: the list of tensors a launch takes, and the walk over its chunks.
+//
+// All of them are streams over memory (0.25 - 1 operation a byte): what bounds them is HBM, for small models the launch.  A launch takes its tensors as
+// kernel arguments (no table in device memory: nothing to allocate, copy or keep, and a captured graph holds all it needs).  The tensors are cut into
+// chunks, numbered through the list; every workgroup takes a run of consecutive chunks and looks a chunk's tensor up with one ballot of the wave for every 64 tensors:
+// lane l holds the first chunk of tensor l (of l + 64, ...).
+#pragma once
+#include <math.h>
+
+#include <algorithm>
+
+#include "gsx_device.hpp"
+#include "../../include/gsx_optim.h"
+
+namespace gsx {
+
+void set_error(const char* msg);
+int check_launch(const char* what);
+
+namespace optim {
+
+// A launch's argument block has room for few tensors (a model's parameter groups) or for many (a network's): the smallest that holds the list is taken.  For
+// 150 tensors one launch of many measured 22 us where five of 32 tensors took 48; the large block costs a launch 2 us on the host.
+constexpr uint32_t kFew = 16, kMany = 256;
+
+// Vectors of four values at any address that the type itself may have: gfx950 loads and stores them with one instruction wherever they lie.
+template <class T> struct Vec4;
+template <> struct Vec4<float> { typedef float type __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct Vec4<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct Vec4<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4), aligned(2))); };
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32_any __attribute__((aligned(1)));
+
+template <class T> GSX_DEV f32x4 load4(const T* p) {   // (of what is not read again soon)
+    return __builtin_convertvector(__builtin_nontemporal_load(reinterpret_cast<const typename Vec4<T>::type*>(p)), f32x4);
+}
+template <class T> GSX_DEV f32x4 load4_keep(const T* p) {   // (of what is)
+    return __builtin_convertvector(*reinterpret_cast<const typename Vec4<T>::type*>(p), f32x4);
+}
+template <class T> GSX_DEV void store4(f32x4 x, T* p) {
+    typedef typename Vec4<T>::type V;
+    __builtin_nontemporal_store((V)__builtin_convertvector(x, V), reinterpret_cast<V*>(p));
+}
+
+// The tensors of a launch and their chunks: begin[i] is the first chunk of tensor i, all ones behind the last tensor.
+template <class R, uint32_t L> struct Chunks {
+    R rec[L];
+    uint32_t begin[L + 1];
+    uint32_t chunks, per;   // of the launch; of a workgroup
+};
+
+// Walks this workgroup's chunks: tensor(rec) for every tensor among them, then chunk(index within the tensor) for each of its chunks.
+template <class R, uint32_t L, class T> GSX_DEV void walk(const Chunks<R, L>& a, T tensor) {
+    uint32_t begin[(L + 63) / 64];
+    const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+    for (uint32_t i = 0; i < (L + 63) / 64; ++i) begin[i] = lane + 64u * i < L ? a.begin[lane + 64u * i] : 0xFFFFFFFFu;
+    uint32_t c = blockIdx.x * a.per;
+    const uint32_t end = std::min(c + a.per, a.chunks);
+    while (c < end) {
+        uint32_t t = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < (L + 63) / 64; ++i) t += (uint32_t)__builtin_popcountll(__ballot(c >= begin[i]));
+        t = __builtin_amdgcn_readfirstlane(t - 1u);
+        const uint32_t first = a.begin[t], stop = std::min(end, a.begin[t + 1]);
+        tensor(a.rec[t], c - first, stop - first);
+        c = stop;
+    }
+}
+
+inline int invalid(const char* msg) { set_error(msg); return GSX_ERR_INVALID_ARGUMENT; }
+inline uint64_t chunks_of(uint64_t n, uint32_t chunk) { return (n + chunk - 1) / chunk; }
+constexpr uint64_t kMostChunks = 0x7FFFFFFFull;   // of a launch
+
+// The number of values of rows x cols, or false where it is beyond what the kernels count.
+inline bool count_of(uint64_t rows, uint64_t cols, uint64_t* n) {
+    if (rows != 0 && cols > (1ull << 40) / rows) return false;
+    *n = rows * cols;
+    return true;
+}
+
+// Gathers tensors and launches them: item(i, &rec, &values) is false for a tensor that does not belong to this launch; launch(list) for every full list.  `few` and
+// `many` are the two argument blocks (host), `grid` the most workgroups of a launch.
+template <class R, class Few, class Many, class Item, class Launch>
+int launch_lists(uint32_t count, uint32_t chunk, uint32_t grid, Few& few, Many& many, Item item, Launch launch) {
+    uint32_t i = 0;
+    while (i < count) {
+        uint32_t k = 0;
+        uint64_t chunks = 0;
+        for (; i < count; ++i) {
+            R rec;
+            uint64_t n = 0;
+            if (!item(i, &rec, &n) || n == 0) continue;
+            if (k == kMany || (k != 0 && chunks + chunks_of(n, chunk) > kMostChunks)) break;
+            if (k < kFew) few.rec[k] = rec, few.begin[k] = (uint32_t)chunks;
+            many.rec[k] = rec;
+            many.begin[k++] = (uint32_t)chunks;
+            chunks += chunks_of(n, chunk);
+        }
+        if (k == 0) break;
+        auto finish = [&](auto& a, uint32_t room) {
+            for (uint32_t j = k; j <= room; ++j) a.begin[j] = 0xFFFFFFFFu;
+            a.chunks = (uint32_t)chunks;
+            a.per = (uint32_t)((chunks + grid - 1) / grid);
+            return launch(a, (uint32_t)((chunks + a.per - 1) / a.per));
+        };
+        const int rc = k <= kFew ? finish(few, kFew) : finish(many, kMany);
+        if (rc != GSX_OK) return rc;
+    }
+    return GSX_OK;
+}
+
+template <class F> void by_dtype(uint32_t d, F f) {
+    if (d == GSX_DTYPE_F32) f(float{});
+    else if (d == GSX_DTYPE_BF16) f(__bf16{});
+    else f(_Float16{});
+}
+
+// ---- AdamW ---------------------------------------------------------------------------------------------------------------------------------------------
+struct Rec {
+    void* param; const void* grad; void* m; void* v; float* m_scale; float* v_scale;
+    uint64_t n, cols, ld_param, ld_grad;
+    uint32_t step, split, flags, ordinal;
+    float bc1, bc2;   // 1 / (1 - beta1^t) and 1 / sqrt(1 - beta2^t) of the step; unused where it is 0: the control block's decides
+    float lr, lr_b, wd, wd_b;
+};
+enum : uint32_t { kHold = 1, kHoldB = 2, kRows = 4 };   // kRows: parameter or gradient is a view whose rows lie apart
+
+struct Betas {
+    const double* control;
+    double log_b1, log_b2;
+    float b1, b1c, b2, b2c, eps;
+    uint32_t seed;
+};
+
+// What the control block says, and the bias corrections of its step: 1 - beta^t = -expm1(t log beta), whose relative error is that of the product (2^-24),
+// where 1 - pow() would lose beta's own rounding (0.999 in 32 bits: 3e-5 of 1 - beta).
+struct Control { bool skip; float factor, bc1, bc2; uint32_t step; };
+GSX_DEV Control control_of(const Betas& a) {
+    Control c = {false, 1.0f, 0.0f, 0.0f, 0u};
+    if (a.control == nullptr) return c;
+    c.skip = a.control[2] != 0.0;
+    c.factor = (float)a.control[1];
+    c.step = std::max((uint32_t)a.control[3], 1u);   // (a block that no norm has advanced: the first step)
+    c.bc1 = 1.0f / -expm1f((float)(a.log_b1 * (double)c.step));
+    c.bc2 = 1.0f / sqrtf(-expm1f((float)(a.log_b2 * (double)c.step)));
+    return c;
+}
+
+struct Rates { float step, step_b, lrwd, lrwd_b, bc2; uint32_t split, flags; };
+GSX_DEV Rates rates_of(const Rec& r, const Control& c) {
+    const float bc1 = r.step ? r.bc1 : c.bc1;
+    return {r.lr * bc1, r.lr_b * bc1, r.lr * r.wd, r.lr_b * r.wd_b, r.step ? r.bc2 : c.bc2, r.split, r.flags};
+}
+
+// The moments as the formulas write them, each product and sum rounded by itself: what is stored in 8 bits is then a function of the inputs that can be
+// computed anywhere to the last bit (a fused product moves a value by 2^-25, and where it lies next to a border of the format, its code by a whole step).
+GSX_DEV float first_moment(const Betas& a, float m, float g) {
+#pragma clang fp contract(off)
+    return a.b1 * m + a.b1c * g;
+}
+GSX_DEV float second_moment(const Betas& a, float v, float g) {
+#pragma clang fp contract(off)
+    return a.b2 * v + a.b2c * g * g;
+}
+
+// Which of the four values that start `q` values behind the start of a row belong to the second column group.
+struct Groups { bool b[4]; };
+GSX_DEV Groups groups_of(uint32_t split, uint32_t q, uint32_t cols) {
+    Groups o = {{false, false, false, false}};
+    if (split) {
+        uint32_t c = q % cols;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            o.b[j] = c >= split;
+            c = c + 1 == cols ? 0 : c + 1;
+        }
+    }
+    return o;
+}
+
+int check_adamw(uint32_t count, const gsx_adamw_tensor* tensors, double beta1, double beta2, double eps, bool eight, const double* control);
+Betas betas_of(double beta1, double beta2, double eps, uint32_t seed, const double* control);
+Rec rec_of(const gsx_adamw_tensor& x, uint32_t ordinal, const Betas& b);
+
+}  // namespace optim
+}  // namespace gsx

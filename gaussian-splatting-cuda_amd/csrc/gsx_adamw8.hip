@@ -1,0 +1,327 @@
+// gsx_adamw8.hip — AdamW over many tensors with moments in 8 bits, and the row selection of such moments (include/gsx_optim.h).
+#include "gsx_adamw.hpp"
+
+namespace gsx {
+namespace optim {
+
+constexpr uint32_t kChunk = 1024;   // values of one pass of a workgroup: four of each lane, 32 lanes to a run
+constexpr uint32_t kGrid = 16384;   // workgroups of a launch at most
+constexpr float kCodeTop = 448.0f, kScaleFloor = 0x1p-120f, kCodeMin = 0x1p-9f;
+static_assert(GSX_MOMENT_RUN == 128, "the exchanges below are among 32 lanes of four values");
+
+GSX_DEV uint32_t mix(uint32_t x) {
+    x ^= x >> 16; x *= 0x9E46A9E5u;
+    x ^= x >> 15; x *= 0xF4B0A2DBu;
+    return x ^ (x >> 16);
+}
+
+template <int C> GSX_DEV float dpp_max(float x) {
+    return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), C, 0xF, 0xF, true)));
+}
+// Largest of the 32 lanes that hold a run (4 values each), in all of them; every lane of the wave takes part.
+GSX_DEV float run_max(float x) {
+    x = dpp_max<0xB1>(x);    // neighbours
+    x = dpp_max<0x4E>(x);    // pairs of a quad
+    x = dpp_max<0x141>(x);   // halves of eight
+    x = dpp_max<0x140>(x);   // halves of a row of 16
+    return fmaxf(x, __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(x), 0x401F)));   // rows of a run
+}
+GSX_DEV float top_of(f32x4 x) {
+    const float top = run_max(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));   // (fmaxf passes over NaN)
+    if (__any(isinf(top))) {   // a run with infinities: the largest of the finite values
+        float f = 0.0f;
+        for (int j = 0; j < 4; ++j) f = fmaxf(f, isinf(x[j]) ? 0.0f : fabsf(x[j]));
+        return run_max(f);
+    }
+    return top;
+}
+GSX_DEV float scale_of(float top) { return fmaxf(top * (1.0f / kCodeTop), kScaleFloor); }
+
+// x / scale to the last bit, by the reciprocal that the four share: the quotient's estimate, what it leaves of x (exact), and the correction that this gives.
+GSX_DEV f32x4 over(f32x4 x, float scale) {
+    const float inv = 1.0f / scale;
+    f32x4 y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float q = x[j] * inv;
+        y[j] = fmaf(-fmaf(q, scale, -x[j]), inv, q);   // (NaN for an infinity too; with these signs -0 stays -0)
+    }
+    return y;
+}
+
+// Four values of a run to their codes.  The hardware's conversions are the definition's: to nearest even, and the stochastic one adds its random word's high
+// 20 bits below the last mantissa bit kept (also in the subnormal codes) and cuts; NaN and infinities become NaN.
+template <bool POSITIVE, bool STOCHASTIC> GSX_DEV uint32_t encode4(f32x4 x, float scale, const uint32_t* u) {
+    f32x4 y = over(x, scale);
+    if (POSITIVE) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = x[j] > 0.0f && y[j] < kCodeMin ? kCodeMin : y[j];
+    }
+    uint32_t w = 0;
+    if (STOCHASTIC) {
+        w = __builtin_amdgcn_cvt_sr_fp8_f32(y.x, u[0], w, 0);
+        w = __builtin_amdgcn_cvt_sr_fp8_f32(y.y, u[1], w, 1);
+        w = __builtin_amdgcn_cvt_sr_fp8_f32(y.z, u[2], w, 2);
+        w = __builtin_amdgcn_cvt_sr_fp8_f32(y.w, u[3], w, 3);
+    } else {
+        w = __builtin_amdgcn_cvt_pk_fp8_f32(y.x, y.y, w, false);
+        w = __builtin_amdgcn_cvt_pk_fp8_f32(y.z, y.w, w, true);
+    }
+    return w;
+}
+GSX_DEV f32x4 decode4(uint32_t w, float scale) {
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    return f32x4{a[0] * scale, a[1] * scale, b[0] * scale, b[1] * scale};
+}
+// Four codes from `off` of `count`: bytes behind the end are zero, and are not touched.
+GSX_DEV uint32_t load_codes(const uint8_t* p, uint32_t off, uint32_t count) {
+    uint32_t w = 0;
+    for (uint32_t j = 0; j < 4 && off + j < count; ++j) w |= (uint32_t)p[off + j] << (8 * j);
+    return w;
+}
+GSX_DEV void store_codes(uint32_t w, uint8_t* p, uint32_t off, uint32_t count) {
+    for (uint32_t j = 0; j < 4 && off + j < count; ++j) p[off + j] = (uint8_t)(w >> (8 * j));
+}
+
+template <uint32_t L> struct List { Chunks<Rec, L> c; Betas b; };
+
+template <class P, class G, bool STOCHASTIC, uint32_t L>
+__global__ __launch_bounds__(256) void adamw8_kernel(List<L> list) {
+    const Betas& a = list.b;
+    const Control ctl = control_of(a);
+    if (ctl.skip) return;
+    walk(list.c, [&](const Rec& r, uint32_t chunk, uint32_t stop) {
+        const Rates k = rates_of(r, ctl);
+        const bool dense = !(k.flags & kRows);
+        const uint64_t n = r.n;
+        const uint32_t cols = (uint32_t)r.cols, off = threadIdx.x * 4u, run = off / GSX_MOMENT_RUN;
+        const uint32_t key = STOCHASTIC ? mix(mix(a.seed + 0x9E3779B9u * (r.step ? r.step : ctl.step)) + 0xC2A6F0B5u * r.ordinal) : 0u;
+        uint64_t base = (uint64_t)chunk * kChunk, row = dense ? 0 : base / r.cols;
+        uint32_t col = k.split || !dense ? (uint32_t)(base % r.cols) : 0;
+        for (; chunk < stop; ++chunk, base += kChunk) {
+            const uint32_t count = (uint32_t)std::min<uint64_t>(n - base, kChunk);
+            const bool whole = dense && count == kChunk;
+            uint8_t* m = (uint8_t*)r.m + base; uint8_t* v = (uint8_t*)r.v + base;
+            float* ms = r.m_scale + base / GSX_MOMENT_RUN; float* vs = r.v_scale + base / GSX_MOMENT_RUN;
+            f32x4 pv = {0, 0, 0, 0}, gv = {0, 0, 0, 0}, mv = {0, 0, 0, 0}, rv = {0, 0, 0, 0};
+            auto at = [&](uint32_t j, uint64_t ld) {   // value off + j of the chunk in a view
+                const uint32_t q = col + off + j, dr = q / cols;
+                return (row + dr) * ld + (q - dr * cols);
+            };
+            if (whole) {
+                const uint32_t mw = __builtin_nontemporal_load(reinterpret_cast<const u32_any*>(m + off)), vw = __builtin_nontemporal_load(reinterpret_cast<const u32_any*>(v + off));
+                gv = load4((const G*)r.grad + base + off);
+                pv = load4((const P*)r.param + base + off);
+                mv = decode4(mw, ms[run]);
+                rv = decode4(vw, vs[run]);
+            } else if (off < count) {
+                mv = decode4(load_codes(m, off, count), ms[run]);
+                rv = decode4(load_codes(v, off, count), vs[run]);
+                for (uint32_t j = 0; j < 4 && off + j < count; ++j) {
+                    gv[j] = (float)((const G*)r.grad)[dense ? base + off + j : at(j, r.ld_grad)];
+                    pv[j] = (float)((const P*)r.param)[dense ? base + off + j : at(j, r.ld_param)];
+                }
+            }
+            // (from here on every lane, also those behind the end: the lanes of a run exchange their largest values)
+            const Groups o = groups_of(k.split, col + off, cols);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (k.flags & (o.b[j] ? kHoldB : kHold)) continue;
+                const float g1 = gv[j] * ctl.factor;
+                mv[j] = first_moment(a, mv[j], g1);
+                rv[j] = sqrtf(second_moment(a, rv[j] * rv[j], g1));
+                pv[j] = pv[j] - (o.b[j] ? k.lrwd_b : k.lrwd) * pv[j] - (o.b[j] ? k.step_b : k.step) * mv[j] / (rv[j] * k.bc2 + a.eps);
+            }
+            const float m_scale = scale_of(top_of(mv)), v_scale = scale_of(top_of(rv));
+            uint32_t um[4], uv[4];
+            if (STOCHASTIC) {
+                const uint32_t i = (uint32_t)base + key + 0x61C8864Fu * (uint32_t)(base >> 32) + off;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const uint32_t w = mix(i + j);
+                    um[j] = w & 0xFFFF0000u;
+                    uv[j] = w << 16;
+                }
+            }
+            const uint32_t mw = encode4<false, STOCHASTIC>(mv, m_scale, um), vw = encode4<true, STOCHASTIC>(rv, v_scale, uv);
+            if (whole) {
+                __builtin_nontemporal_store(mw, reinterpret_cast<u32_any*>(m + off));
+                __builtin_nontemporal_store(vw, reinterpret_cast<u32_any*>(v + off));
+                store4(pv, (P*)r.param + base + off);
+            } else if (off < count) {
+                store_codes(mw, m, off, count);
+                store_codes(vw, v, off, count);
+                for (uint32_t j = 0; j < 4 && off + j < count; ++j)
+                    if (!(k.flags & (o.b[j] ? kHoldB : kHold))) ((P*)r.param)[dense ? base + off + j : at(j, r.ld_param)] = (P)pv[j];
+            }
+            if (off < count && (off & (GSX_MOMENT_RUN - 1)) == 0) { ms[run] = m_scale; vs[run] = v_scale; }
+            if (k.split || !dense) {
+                const uint32_t q = col + kChunk;
+                row += dense ? 0 : q / cols;
+                col = q % cols;
+            }
+        }
+    });
+}
+
+// ---- rows of 8-bit moments --------------------------------------------------------------------------------------------------------------------------------
+struct SelectRec { const uint8_t *m, *v; const float *ms, *vs; uint8_t *mo, *vo; float *mso, *vso; uint64_t cols; };
+template <uint32_t L> struct SelectList {
+    Chunks<SelectRec, L> c;
+    const int64_t* index;
+    uint64_t rows_in, rows_out;
+};
+
+constexpr uint32_t kSelect = 2048;   // values of one pass of a workgroup
+
+// A chunk of the new moments is gathered into LDS in pieces of up to four values of one row (an index, two codes words and two scales a piece, whatever the rows' length and
+// the places where old and new runs begin), then coded from there like the update's.
+template <uint32_t L> __global__ __launch_bounds__(256) void select_rows_kernel(SelectList<L> a) {
+    __shared__ float lds[2][kSelect];
+    walk(a.c, [&](const SelectRec& r, uint32_t chunk, uint32_t stop) {
+        const uint32_t cols = (uint32_t)r.cols, pieces = (cols + 3) / 4;
+        const uint64_t n = a.rows_out * r.cols, n_in = a.rows_in * r.cols;
+        for (; chunk < stop; ++chunk) {
+            const uint64_t base = (uint64_t)chunk * kSelect, row0 = base / r.cols;
+            const uint32_t count = (uint32_t)std::min<uint64_t>(n - base, kSelect);
+            const uint32_t col0 = (uint32_t)(base - row0 * r.cols);
+            const uint32_t first = col0 / 4, items = (uint32_t)(((uint64_t)col0 + count + cols - 1) / cols) * pieces;   // (of all rows that the chunk touches)
+            __syncthreads();
+            for (uint32_t i = first + threadIdx.x; i < items; i += 256u) {
+                const uint32_t dr = i / pieces, c = (i - dr * pieces) * 4u, len = std::min(cols - c, 4u);
+                const int64_t to = (int64_t)dr * cols + c - col0;   // where in the chunk; a piece may start before it and end behind it
+                if (to >= (int64_t)count) break;
+                const int64_t src = a.index[row0 + dr];
+                f32x4 mv = {0, 0, 0, 0}, rv = {0, 0, 0, 0};
+                if (src >= 0 && (uint64_t)src < a.rows_in) {
+                    const uint64_t at = (uint64_t)src * cols + c;
+                    const uint64_t s0 = at / GSX_MOMENT_RUN, s1 = (at + len - 1) / GSX_MOMENT_RUN;
+                    uint32_t mw, vw;
+                    if (at + 4 <= n_in) {
+                        mw = *reinterpret_cast<const u32_any*>(r.m + at);
+                        vw = *reinterpret_cast<const u32_any*>(r.v + at);
+                    } else {
+                        mw = load_codes(r.m + at, 0, len);
+                        vw = load_codes(r.v + at, 0, len);
+                    }
+                    mv = decode4(mw, 1.0f);
+                    rv = decode4(vw, 1.0f);
+                    const float ms = r.ms[s0], vs = r.vs[s0];
+                    float ms1 = ms, vs1 = vs;
+                    if (s1 != s0) { ms1 = r.ms[s1]; vs1 = r.vs[s1]; }
+                    const uint32_t left = GSX_MOMENT_RUN - (uint32_t)(at % GSX_MOMENT_RUN);   // values up to the next run
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        mv[j] *= j < left ? ms : ms1;
+                        rv[j] *= j < left ? vs : vs1;
+                    }
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    if (j < len && to + j >= 0 && to + j < (int64_t)count) {
+                        lds[0][to + j] = mv[j];
+                        lds[1][to + j] = rv[j];
+                    }
+                }
+            }
+            __syncthreads();
+            for (uint32_t pass = 0; pass < kSelect; pass += 1024u) {   // (the same number of passes for every lane: the runs' lanes exchange their largest values)
+                const uint32_t off = pass + threadIdx.x * 4u;
+                f32x4 mv, rv;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    mv[j] = off + j < count ? lds[0][off + j] : 0.0f;
+                    rv[j] = off + j < count ? lds[1][off + j] : 0.0f;
+                }
+                const float m_scale = scale_of(top_of(mv)), v_scale = scale_of(top_of(rv));
+                if (off >= count) continue;
+                const uint32_t mw = encode4<false, false>(mv, m_scale, nullptr), vw = encode4<true, false>(rv, v_scale, nullptr);
+                if (off + 4 <= count) {
+                    *reinterpret_cast<u32_any*>(r.mo + base + off) = mw;
+                    *reinterpret_cast<u32_any*>(r.vo + base + off) = vw;
+                } else {
+                    store_codes(mw, r.mo + base, off, count);
+                    store_codes(vw, r.vo + base, off, count);
+                }
+                if ((off & (GSX_MOMENT_RUN - 1)) == 0) { r.mso[(base + off) / GSX_MOMENT_RUN] = m_scale; r.vso[(base + off) / GSX_MOMENT_RUN] = v_scale; }
+            }
+        }
+    });
+}
+
+}  // namespace optim
+}  // namespace gsx
+
+using namespace gsx;
+using namespace gsx::optim;
+
+extern "C" int gsx_adamw8_step_multi(uint32_t count, const gsx_adamw_tensor* tensors, double beta1, double beta2, double eps, int stochastic, uint32_t seed,
+                                     const double* control, void* stream) {
+    const int bad = check_adamw(count, tensors, beta1, beta2, eps, true, control);
+    if (bad != GSX_OK || count == 0) return bad;
+    List<kFew> few;
+    List<kMany> many;
+    few.b = many.b = betas_of(beta1, beta2, eps, seed, control);
+    for (uint32_t types = 0; types < 9; ++types) {
+        const uint32_t pd = types / 3, gd = types % 3;
+        const int rc = launch_lists<Rec>(
+            count, kChunk, kGrid, few.c, many.c,
+            [&](uint32_t i, Rec* r, uint64_t* n) {
+                if (tensors[i].param_dtype != pd || tensors[i].grad_dtype != gd) return false;
+                *r = rec_of(tensors[i], i, few.b);
+                *n = r->n;
+                return true;
+            },
+            [&](auto& c, uint32_t blocks) {
+                auto launch = [&](auto& a, auto p, auto g, auto rounding) {
+                    constexpr uint32_t L = sizeof(a.c.rec) / sizeof(Rec);
+                    hipLaunchKernelGGL((adamw8_kernel<decltype(p), decltype(g), decltype(rounding)::value, L>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
+                };
+                by_dtype(pd, [&](auto p) {
+                    by_dtype(gd, [&](auto g) {
+                        auto list = [&](auto& a) {
+                            if (stochastic) launch(a, p, g, std::true_type{});
+                            else launch(a, p, g, std::false_type{});
+                        };
+                        if constexpr (sizeof(c.rec) == sizeof(few.c.rec)) list(few);
+                        else list(many);
+                    });
+                });
+                return check_launch("adamw8_step_multi");
+            });
+        if (rc != GSX_OK) return rc;
+    }
+    return GSX_OK;
+}
+
+extern "C" int gsx_adamw8_select_rows(uint32_t count, const gsx_moments8* tensors, uint64_t rows_in, uint64_t rows_out, const int64_t* index, void* stream) {
+    if (count == 0 || rows_out == 0) return GSX_OK;
+    if (tensors == nullptr || index == nullptr) return invalid("adamw8_select_rows: null list or index");
+    for (uint32_t i = 0; i < count; ++i) {
+        const gsx_moments8& x = tensors[i];
+        uint64_t n;
+        if (!count_of(rows_in, x.cols, &n) || !count_of(rows_out, x.cols, &n) || x.cols > (1ull << 31)) return invalid("adamw8_select_rows: tensor too large");
+        if (x.cols == 0) continue;
+        if (!x.avg_out || !x.rms_out || !x.avg_scale_out || !x.rms_scale_out) return invalid("adamw8_select_rows: null tensor");
+        if (rows_in != 0 && (!x.avg_in || !x.rms_in || !x.avg_scale_in || !x.rms_scale_in)) return invalid("adamw8_select_rows: null tensor");
+    }
+    SelectList<kFew> few;
+    SelectList<kMany> many;
+    few.index = many.index = index;
+    few.rows_in = many.rows_in = rows_in;
+    few.rows_out = many.rows_out = rows_out;
+    return launch_lists<SelectRec>(
+        count, kSelect, kGrid, few.c, many.c,
+        [&](uint32_t i, SelectRec* r, uint64_t* n) {
+            const gsx_moments8& x = tensors[i];
+            *r = SelectRec{(const uint8_t*)x.avg_in, (const uint8_t*)x.rms_in, x.avg_scale_in, x.rms_scale_in, (uint8_t*)x.avg_out, (uint8_t*)x.rms_out,
+                           x.avg_scale_out, x.rms_scale_out, x.cols};
+            *n = rows_out * x.cols;
+            return true;
+        },
+        [&](auto& c, uint32_t blocks) {
+            if constexpr (sizeof(c.rec) == sizeof(few.c.rec)) hipLaunchKernelGGL(select_rows_kernel<kFew>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, few);
+            else hipLaunchKernelGGL(select_rows_kernel<kMany>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, many);
+            return check_launch("adamw8_select_rows");
+        });
+}
