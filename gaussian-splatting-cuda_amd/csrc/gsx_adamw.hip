@@ -9,11 +9,6 @@ constexpr uint32_t kGrid = 16384;   // workgroups of a launch at most
 
 template <uint32_t L> struct List { Chunks<Rec, L> c; Betas b; };
 
-// One parameter's step, after its moments (root: sqrt(v)).
-GSX_DEV float stepped(const Betas& a, const Rates& k, bool b, float p, float m, float root) {
-    return p - (b ? k.lrwd_b : k.lrwd) * p - (b ? k.step_b : k.step) * m / (root * k.bc2 + a.eps);
-}
-
 template <class P, class G, uint32_t L>
 __global__ __launch_bounds__(256) void adamw_kernel(List<L> list) {
     const Betas& a = list.b;
@@ -21,77 +16,70 @@ __global__ __launch_bounds__(256) void adamw_kernel(List<L> list) {
     if (ctl.skip) return;
     walk(list.c, [&](const Rec& r, uint32_t chunk, uint32_t stop) {
         const Rates k = rates_of(r, ctl);
-        const uint64_t n = r.n;
-        const uint32_t cols = (uint32_t)r.cols;
-        uint64_t base = (uint64_t)chunk * kChunk;
-        if (!(k.flags & kRows)) {
-            uint32_t col0 = k.split ? (uint32_t)(base % r.cols) : 0;
-            for (; chunk < stop; ++chunk, base += kChunk) {
-                const uint32_t count = (uint32_t)std::min<uint64_t>(n - base, kChunk), off = threadIdx.x * 4u;
-                P* p = (P*)r.param + base; const G* g = (const G*)r.grad + base;
-                float* m = (float*)r.m + base; float* v = (float*)r.v + base;
-                if (off + 4 <= count) {
-                    f32x4 gv = load4(g + off), mv = load4(m + off), vv = load4(v + off), pv = load4(p + off);
-                    const Groups o = groups_of(k.split, col0 + off, cols);
+        Place at(r, k.split, (uint64_t)chunk * kChunk, kChunk);
+        auto pass = [&](auto whole) {   // (compiled twice: the ends of tensors and the views stay out of the way of the whole chunks)
+            const uint32_t off = threadIdx.x * 4u;
+            float* m = (float*)r.m + at.base; float* v = (float*)r.v + at.base;
+            f32x4 pv, gv, mv, vv;
+            if constexpr (whole.value) {
+                gv = load4((const G*)r.grad + at.base + off);
+                mv = load4(m + off);
+                vv = load4(v + off);
+                pv = load4((const P*)r.param + at.base + off);
+            } else {   // the end of a tensor, or a view: value by value, all loads at once, none behind the end
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (k.flags & (o.b[j] ? kHoldB : kHold)) continue;
-                        const float g1 = gv[j] * ctl.factor;
-                        mv[j] = a.b1 * mv[j] + a.b1c * g1;
-                        vv[j] = a.b2 * vv[j] + a.b2c * g1 * g1;
-                        pv[j] = stepped(a, k, o.b[j], pv[j], mv[j], sqrtf(vv[j]));
-                    }
-                    store4(mv, m + off); store4(vv, v + off); store4(pv, p + off);
-                } else {   // the last one to three values of the tensor
-                    for (uint32_t i = off; i < count; ++i) {
-                        const bool b = k.split && (col0 + i) % cols >= k.split;
-                        if (k.flags & (b ? kHoldB : kHold)) continue;
-                        const float g1 = (float)g[i] * ctl.factor;
-                        const float m1 = a.b1 * m[i] + a.b1c * g1, v1 = a.b2 * v[i] + a.b2c * g1 * g1;
-                        p[i] = (P)stepped(a, k, b, (float)p[i], m1, sqrtf(v1));
-                        m[i] = m1;
-                        v[i] = v1;
-                    }
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const uint32_t i = std::min(off + j, at.count - 1u);
+                    gv[j] = (float)((const G*)r.grad)[at(i, r.ld_grad)];
+                    pv[j] = (float)((const P*)r.param)[at(i, r.ld_param)];
+                    mv[j] = m[i];
+                    vv[j] = v[i];
                 }
-                if (k.split) col0 = (col0 + kChunk) % cols;
             }
-            return;
-        }
-        // a view: one value of a lane at a time
-        const uint64_t row0 = base / r.cols;
-        uint64_t row = row0;
-        uint32_t col = (uint32_t)(base - row0 * r.cols);
-        for (; chunk < stop; ++chunk, base += kChunk) {
-            const uint32_t count = (uint32_t)std::min<uint64_t>(n - base, kChunk);
-            float* m = (float*)r.m + base; float* v = (float*)r.v + base;
-            for (uint32_t off = threadIdx.x; off < count; off += 256u) {
-                const uint32_t q = col + off, dr = q / cols, c = q - dr * cols;
-                const bool b = k.split && c >= k.split;
-                if (k.flags & (b ? kHoldB : kHold)) continue;
-                P* p = (P*)r.param + ((row + dr) * r.ld_param + c);
-                const float g1 = (float)((const G*)r.grad)[(row + dr) * r.ld_grad + c] * ctl.factor;
-                const float m1 = a.b1 * m[off] + a.b1c * g1, v1 = a.b2 * v[off] + a.b2c * g1 * g1;
-                *p = (P)stepped(a, k, b, (float)*p, m1, sqrtf(v1));
-                m[off] = m1;
-                v[off] = v1;
+            const Groups o = groups_of(k.split, at.col + off, at.cols);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (k.flags & (o.b[j] ? kHoldB : kHold)) continue;
+                const float g1 = gv[j] * ctl.factor;
+                mv[j] = a.b1 * mv[j] + a.b1c * g1;
+                vv[j] = a.b2 * vv[j] + a.b2c * g1 * g1;
+                pv[j] = stepped(a, k, o.b[j], pv[j], mv[j], sqrtf(vv[j]));
             }
-            const uint32_t q = col + kChunk;
-            row += q / cols;
-            col = q % cols;
+            if constexpr (whole.value) {
+                store4(mv, m + off);
+                store4(vv, v + off);
+                store4(pv, (P*)r.param + at.base + off);
+            } else {
+                for (uint32_t j = 0; j < 4 && off + j < at.count; ++j) {
+                    if (k.flags & (o.b[j] ? kHoldB : kHold)) continue;
+                    ((P*)r.param)[at(off + j, r.ld_param)] = (P)pv[j];
+                    m[off + j] = mv[j];
+                    v[off + j] = vv[j];
+                }
+            }
+        };
+        for (; chunk < stop; ++chunk, at.next(kChunk)) {
+            if (at.whole) pass(std::true_type{});
+            else pass(std::false_type{});
         }
     });
 }
 
 // ---- the norm ----------------------------------------------------------------------------------------------------------------------------------------
-constexpr uint32_t kNormVecs = 4, kNormChunk = 1024 * kNormVecs, kNormGrid = 2048;   // (few partial sums for the last workgroup)
+constexpr uint32_t kNormVecs = 4, kNormChunk = 1024 * kNormVecs, kNormGrid = 2048;
+// Up to this many workgroups the last one to finish adds the sums up; every one costs 45 ns there (an atomic on one word, and what the release before it
+// waits for: 2 048 of them took 100 of 284 us), a launch of its own 3 us.
+constexpr uint32_t kTickets = 64;
+// Gradients that fit the last-level cache (256 MB) are read to stay there for the update behind the norm: 1 M splats, norm and update 314 us (352 without).  Larger ones
+// stream past it: 295 M values 6.2 TB/s, 5.6 without.
+constexpr uint64_t kCacheBytes = 256ull << 20;
 
 struct NormRec { const void* grad; uint64_t n, cols, ld; };
+struct NormEnd { double* partial; double* control; double max_norm; uint32_t blocks; };   // partial: one for each workgroup of the whole call
 template <uint32_t L> struct NormList {
     Chunks<NormRec, L> c;
-    double* partial;   // of the whole call: one for each workgroup
-    double* control;
-    double max_norm;
-    uint32_t first, blocks;   // this launch's first partial; workgroups of the whole call
+    NormEnd e;
+    uint32_t first;   // this launch's first partial
 };
 
 GSX_DEV double block_sum(double x, double* lds) {
@@ -102,9 +90,23 @@ GSX_DEV double block_sum(double x, double* lds) {
     return (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
-// Sums of squares in 64 bits: no square of a 32-bit number overflows, so the sum is finite exactly if all gradients are.  Every workgroup leaves its sum, the
-// last one to finish adds them up in their order (the same bits every time) and writes the control block.
-template <class G, uint32_t L>
+// One workgroup adds the partial sums up in their order (the same bits every time) and writes the control block.
+GSX_DEV void norm_end(const NormEnd& e, double* lds) {
+    double total = 0.0;
+    for (uint32_t i = threadIdx.x; i < e.blocks; i += 256u) total += __hip_atomic_load(e.partial + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    total = block_sum(total, lds);
+    if (threadIdx.x == 0) {
+        const bool fine = isfinite(total);
+        const double norm = sqrt(total);
+        e.control[0] = norm;
+        e.control[1] = fine ? fmin(1.0, e.max_norm / (norm + 1e-6)) : 0.0;
+        e.control[2] = fine ? 0.0 : 1.0;
+        e.control[3] += fine ? 1.0 : 0.0;
+    }
+}
+
+// Sums of squares in 64 bits: no square of a 32-bit number overflows, so the sum is finite exactly if all gradients are.
+template <class G, uint32_t L, bool KEEP>
 __global__ __launch_bounds__(256) void grad_norm_kernel(NormList<L> a) {
     __shared__ double lds[4];
     __shared__ uint32_t last;
@@ -121,14 +123,16 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(NormList<L> a) {
 #pragma unroll
                 for (uint32_t u = 0; u < kNormVecs; ++u) {
                     const uint32_t off = (u * 256u + threadIdx.x) * 4u;
-                    x[u] = off + 4 <= count ? load4_keep(g + off) : f32x4{0, 0, 0, 0};
+                    x[u] = off + 4 > count ? f32x4{0, 0, 0, 0} : KEEP ? load4_keep(g + off) : load4(g + off);
                 }
 #pragma unroll
                 for (uint32_t u = 0; u < kNormVecs; ++u)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) sum = fma((double)x[u][j], (double)x[u][j], sum);
-                const uint32_t rest = (count & ~3u) + threadIdx.x;   // the last one to three values of the tensor
-                if (rest < count) { const double x1 = (double)(float)g[rest]; sum = fma(x1, x1, sum); }
+                if (const uint32_t rest = count & 3u; rest != 0 && threadIdx.x < rest) {   // the last one to three values of the tensor
+                    const double x1 = (double)(float)g[(count & ~3u) + threadIdx.x];
+                    sum = fma(x1, x1, sum);
+                }
             } else {
                 const uint64_t row = base / r.cols;
                 const uint32_t col = (uint32_t)(base - row * r.cols), cols = (uint32_t)r.cols;
@@ -141,25 +145,20 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(NormList<L> a) {
         }
     });
     sum = block_sum(sum, lds);
-    uint32_t* ticket = reinterpret_cast<uint32_t*>(a.control + 4);
+    uint32_t* ticket = reinterpret_cast<uint32_t*>(a.e.control + 4);
     if (threadIdx.x == 0) {
-        __hip_atomic_store(a.partial + a.first + blockIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.blocks - 1u;
+        __hip_atomic_store(a.e.partial + a.first + blockIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = a.e.blocks <= kTickets && __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.e.blocks - 1u;
     }
     __syncthreads();
     if (!last) return;
-    double total = 0.0;
-    for (uint32_t i = threadIdx.x; i < a.blocks; i += 256u) total += __hip_atomic_load(a.partial + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    total = block_sum(total, lds);
-    if (threadIdx.x == 0) {
-        const bool fine = isfinite(total);
-        const double norm = sqrt(total);
-        a.control[0] = norm;
-        a.control[1] = fine ? fmin(1.0, a.max_norm / (norm + 1e-6)) : 0.0;
-        a.control[2] = fine ? 0.0 : 1.0;
-        a.control[3] += fine ? 1.0 : 0.0;
-        __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+    norm_end(a.e, lds);
+    if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__global__ __launch_bounds__(256) void grad_norm_end_kernel(NormEnd e) {
+    __shared__ double lds[4];
+    norm_end(e, lds);
 }
 
 // Calls f(list, workgroups, dtype) for every launch of a norm over these tensors; what the lists hold besides the tensors is f's.
@@ -232,11 +231,13 @@ Betas betas_of(double beta1, double beta2, double eps, uint32_t seed, const doub
     return Betas{control, log(beta1), log(beta2), (float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, seed};
 }
 
-Rec rec_of(const gsx_adamw_tensor& x, uint32_t ordinal, const Betas& b) {
+Rec rec_of(const gsx_adamw_tensor& x, uint32_t ordinal, const Betas& b, Corrections* last) {
+    if (last->step != x.step || last->step == 0)   // (the tensors of a list mostly share their step)
+        *last = Corrections{x.step, (float)(1.0 / -expm1(b.log_b1 * (double)x.step)), (float)(1.0 / sqrt(-expm1(b.log_b2 * (double)x.step)))};
     const bool dense = x.rows <= 1 || (x.ld_param == x.cols && x.ld_grad == x.cols);
     return Rec{x.param, x.grad, x.exp_avg, x.exp_avg_sq, x.avg_scale, x.rms_scale, x.rows * x.cols, x.cols, x.ld_param, x.ld_grad, (uint32_t)x.step, x.split,
-               (x.hold ? kHold : 0u) | (x.hold_b ? kHoldB : 0u) | (dense ? 0u : kRows), ordinal, (float)(1.0 / -expm1(b.log_b1 * (double)x.step)),
-               (float)(1.0 / sqrt(-expm1(b.log_b2 * (double)x.step))), x.lr, x.lr_b, x.weight_decay, x.weight_decay_b};
+               (x.hold ? kHold : 0u) | (x.hold_b ? kHoldB : 0u) | (dense ? 0u : kRows), ordinal, last->bc1, last->bc2, x.lr, x.lr_b, x.weight_decay,
+               x.weight_decay_b};
 }
 
 }  // namespace optim
@@ -254,13 +255,14 @@ extern "C" int gsx_adamw_step_multi(uint32_t count, const gsx_adamw_tensor* tens
     List<kFew> few;
     List<kMany> many;
     few.b = many.b = betas_of(beta1, beta2, eps, 0, control);
+    Corrections last = {};
     for (uint32_t types = 0; types < 9; ++types) {
         const uint32_t pd = types / 3, gd = types % 3;
         const int rc = launch_lists<Rec>(
             count, kChunk, kGrid, few.c, many.c,
             [&](uint32_t i, Rec* r, uint64_t* n) {
                 if (tensors[i].param_dtype != pd || tensors[i].grad_dtype != gd) return false;
-                *r = rec_of(tensors[i], i, few.b);
+                *r = rec_of(tensors[i], i, few.b, &last);
                 *n = r->n;
                 return true;
             },
@@ -295,22 +297,30 @@ extern "C" int gsx_grad_norm_multi(uint32_t count, const gsx_grad_tensor* tensor
     if (control == nullptr || workspace == nullptr) return invalid("grad_norm_multi: null control block or workspace");
     const uint32_t blocks = norm_blocks(count, tensors);
     if (workspace_bytes < blocks * sizeof(double)) { set_error("grad_norm_multi: workspace too small"); return GSX_ERR_WORKSPACE_TOO_SMALL; }
+    uint64_t bytes = 0;
+    for (uint32_t i = 0; i < count; ++i) bytes += tensors[i].rows * tensors[i].cols * (tensors[i].dtype == GSX_DTYPE_F32 ? 4 : 2);
+    const NormEnd end = {(double*)workspace, control, max_norm, blocks};
     uint32_t first = 0;
     auto launch = [&](auto& a, uint32_t grid, uint32_t d) {
-        a.partial = (double*)workspace; a.control = control; a.max_norm = max_norm; a.first = first; a.blocks = blocks;
+        a.e = end; a.first = first;
         by_dtype(d, [&](auto g) {
             typedef decltype(g) G;
             constexpr uint32_t L = sizeof(a.c.rec) / sizeof(NormRec);
-            hipLaunchKernelGGL((grad_norm_kernel<G, L>), dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
+            if (bytes <= kCacheBytes) hipLaunchKernelGGL((grad_norm_kernel<G, L, true>), dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
+            else hipLaunchKernelGGL((grad_norm_kernel<G, L, false>), dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
         });
         first += grid;
         return check_launch("grad_norm_multi");
     };
-    const int rc = norm_lists(count, tensors, launch);
-    if (rc != GSX_OK || first != 0) return rc;
-    NormList<kFew> none;   // nothing to add up: the norm is zero
-    for (uint32_t j = 0; j <= kFew; ++j) none.c.begin[j] = 0xFFFFFFFFu;
-    none.c.chunks = 0;
-    none.c.per = 1;
-    return launch(none, 1, GSX_DTYPE_F32);
+    int rc = norm_lists(count, tensors, launch);
+    if (rc == GSX_OK && first == 0) {   // nothing to add up: the norm is zero
+        NormList<kFew> none;
+        for (uint32_t j = 0; j <= kFew; ++j) none.c.begin[j] = 0xFFFFFFFFu;
+        none.c.chunks = 0;
+        none.c.per = 1;
+        rc = launch(none, 1, GSX_DTYPE_F32);
+    }
+    if (rc != GSX_OK || blocks <= kTickets) return rc;
+    hipLaunchKernelGGL(grad_norm_end_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, end);
+    return check_launch("grad_norm_multi");
 }

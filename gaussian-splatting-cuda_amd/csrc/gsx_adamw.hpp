@@ -179,9 +179,52 @@ GSX_DEV Groups groups_of(uint32_t split, uint32_t q, uint32_t cols) {
     return o;
 }
 
+// One parameter's step, after its moments (root: sqrt(v)).
+GSX_DEV float stepped(const Betas& a, const Rates& k, bool b, float p, float m, float root) {
+    return p - (b ? k.lrwd_b : k.lrwd) * p - (b ? k.step_b : k.step) * m / (root * k.bc2 + a.eps);
+}
+
+// Where the values of a chunk lie.  Rows and columns are followed from chunk to chunk, and only where something goes by them.
+struct Place {
+    const uint64_t n;
+    const uint32_t cols;
+    const bool view, by_column;
+    uint64_t base, row = 0;   // first value of the chunk, and its row (of a view)
+    uint32_t col = 0, count;  // its column; values in the chunk
+    bool whole;               // all values of the chunk, one behind the other in all of the tensor's arrays
+    GSX_DEV Place(const Rec& r, uint32_t split, uint64_t first, uint32_t chunk)
+        : n(r.n), cols((uint32_t)r.cols), view(r.flags & kRows), by_column(split || view), base(first) {
+        if (by_column) {
+            row = base / r.cols;
+            col = (uint32_t)(base - row * r.cols);
+        }
+        size(chunk);
+    }
+    GSX_DEV void size(uint32_t chunk) {
+        count = (uint32_t)std::min<uint64_t>(n - base, chunk);
+        whole = !view && count == chunk;
+    }
+    GSX_DEV void next(uint32_t chunk) {
+        base += chunk;
+        if (by_column) {
+            const uint32_t q = col + chunk, dr = q / cols;
+            row += dr;
+            col = q - dr * cols;
+        }
+        size(chunk);   // (behind the last chunk: not used)
+    }
+    // Where value i of the chunk is in an array whose rows are ld apart if the tensor is a view.
+    GSX_DEV uint64_t operator()(uint32_t i, uint64_t ld) const {
+        if (!view) return base + i;
+        const uint32_t q = col + i, dr = q / cols;
+        return (row + dr) * ld + (q - dr * cols);
+    }
+};
+
+struct Corrections { uint64_t step; float bc1, bc2; };
 int check_adamw(uint32_t count, const gsx_adamw_tensor* tensors, double beta1, double beta2, double eps, bool eight, const double* control);
 Betas betas_of(double beta1, double beta2, double eps, uint32_t seed, const double* control);
-Rec rec_of(const gsx_adamw_tensor& x, uint32_t ordinal, const Betas& b);
+Rec rec_of(const gsx_adamw_tensor& x, uint32_t ordinal, const Betas& b, Corrections* last);
 
 }  // namespace optim
 }  // namespace gsx

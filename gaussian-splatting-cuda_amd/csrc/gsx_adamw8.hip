@@ -73,10 +73,14 @@ GSX_DEV f32x4 decode4(uint32_t w, float scale) {
     const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
     return f32x4{a[0] * scale, a[1] * scale, b[0] * scale, b[1] * scale};
 }
-// Four codes from `off` of `count`: bytes behind the end are zero, and are not touched.
+// Four codes from `off` of `count` > 0: those behind the end are zero.  (Four loads at once, none of them behind the end, instead of one after the other.)
 GSX_DEV uint32_t load_codes(const uint8_t* p, uint32_t off, uint32_t count) {
     uint32_t w = 0;
-    for (uint32_t j = 0; j < 4 && off + j < count; ++j) w |= (uint32_t)p[off + j] << (8 * j);
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t c = p[std::min(off + j, count - 1u)];
+        w |= off + j < count ? c << (8 * j) : 0u;
+    }
     return w;
 }
 GSX_DEV void store_codes(uint32_t w, uint8_t* p, uint32_t off, uint32_t count) {
@@ -92,50 +96,45 @@ __global__ __launch_bounds__(256) void adamw8_kernel(List<L> list) {
     if (ctl.skip) return;
     walk(list.c, [&](const Rec& r, uint32_t chunk, uint32_t stop) {
         const Rates k = rates_of(r, ctl);
-        const bool dense = !(k.flags & kRows);
-        const uint64_t n = r.n;
-        const uint32_t cols = (uint32_t)r.cols, off = threadIdx.x * 4u, run = off / GSX_MOMENT_RUN;
+        const uint32_t off = threadIdx.x * 4u, run = off / GSX_MOMENT_RUN;
         const uint32_t key = STOCHASTIC ? mix(mix(a.seed + 0x9E3779B9u * (r.step ? r.step : ctl.step)) + 0xC2A6F0B5u * r.ordinal) : 0u;
-        uint64_t base = (uint64_t)chunk * kChunk, row = dense ? 0 : base / r.cols;
-        uint32_t col = k.split || !dense ? (uint32_t)(base % r.cols) : 0;
-        for (; chunk < stop; ++chunk, base += kChunk) {
-            const uint32_t count = (uint32_t)std::min<uint64_t>(n - base, kChunk);
-            const bool whole = dense && count == kChunk;
-            uint8_t* m = (uint8_t*)r.m + base; uint8_t* v = (uint8_t*)r.v + base;
-            float* ms = r.m_scale + base / GSX_MOMENT_RUN; float* vs = r.v_scale + base / GSX_MOMENT_RUN;
-            f32x4 pv = {0, 0, 0, 0}, gv = {0, 0, 0, 0}, mv = {0, 0, 0, 0}, rv = {0, 0, 0, 0};
-            auto at = [&](uint32_t j, uint64_t ld) {   // value off + j of the chunk in a view
-                const uint32_t q = col + off + j, dr = q / cols;
-                return (row + dr) * ld + (q - dr * cols);
-            };
-            if (whole) {
+        Place at(r, k.split, (uint64_t)chunk * kChunk, kChunk);
+        auto pass = [&](auto whole) {   // (compiled twice: the ends of tensors and the views stay out of the way of the whole chunks)
+            uint8_t* m = (uint8_t*)r.m + at.base; uint8_t* v = (uint8_t*)r.v + at.base;
+            float* ms = r.m_scale + at.base / GSX_MOMENT_RUN; float* vs = r.v_scale + at.base / GSX_MOMENT_RUN;
+            f32x4 pv, gv, mv, rv;
+            if constexpr (whole.value) {
                 const uint32_t mw = __builtin_nontemporal_load(reinterpret_cast<const u32_any*>(m + off)), vw = __builtin_nontemporal_load(reinterpret_cast<const u32_any*>(v + off));
-                gv = load4((const G*)r.grad + base + off);
-                pv = load4((const P*)r.param + base + off);
+                gv = load4((const G*)r.grad + at.base + off);
+                pv = load4((const P*)r.param + at.base + off);
                 mv = decode4(mw, ms[run]);
                 rv = decode4(vw, vs[run]);
-            } else if (off < count) {
-                mv = decode4(load_codes(m, off, count), ms[run]);
-                rv = decode4(load_codes(v, off, count), vs[run]);
-                for (uint32_t j = 0; j < 4 && off + j < count; ++j) {
-                    gv[j] = (float)((const G*)r.grad)[dense ? base + off + j : at(j, r.ld_grad)];
-                    pv[j] = (float)((const P*)r.param)[dense ? base + off + j : at(j, r.ld_param)];
+            } else {   // the end of a tensor, or a view: value by value, all loads at once, none behind the end
+                const uint32_t mw = load_codes(m, off, at.count), vw = load_codes(v, off, at.count), here = std::min(off, at.count - 1u) / GSX_MOMENT_RUN;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const uint32_t i = std::min(off + j, at.count - 1u);
+                    const float g1 = (float)((const G*)r.grad)[at(i, r.ld_grad)];
+                    gv[j] = off + j < at.count ? g1 : 0.0f;
+                    pv[j] = (float)((const P*)r.param)[at(i, r.ld_param)];
                 }
+                mv = decode4(mw, ms[here]);
+                rv = decode4(vw, vs[here]);
             }
             // (from here on every lane, also those behind the end: the lanes of a run exchange their largest values)
-            const Groups o = groups_of(k.split, col + off, cols);
+            const Groups o = groups_of(k.split, at.col + off, at.cols);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (k.flags & (o.b[j] ? kHoldB : kHold)) continue;
                 const float g1 = gv[j] * ctl.factor;
                 mv[j] = first_moment(a, mv[j], g1);
                 rv[j] = sqrtf(second_moment(a, rv[j] * rv[j], g1));
-                pv[j] = pv[j] - (o.b[j] ? k.lrwd_b : k.lrwd) * pv[j] - (o.b[j] ? k.step_b : k.step) * mv[j] / (rv[j] * k.bc2 + a.eps);
+                pv[j] = stepped(a, k, o.b[j], pv[j], mv[j], rv[j]);
             }
             const float m_scale = scale_of(top_of(mv)), v_scale = scale_of(top_of(rv));
             uint32_t um[4], uv[4];
             if (STOCHASTIC) {
-                const uint32_t i = (uint32_t)base + key + 0x61C8864Fu * (uint32_t)(base >> 32) + off;
+                const uint32_t i = (uint32_t)at.base + key + 0x61C8864Fu * (uint32_t)(at.base >> 32) + off;
 #pragma unroll
                 for (uint32_t j = 0; j < 4; ++j) {
                     const uint32_t w = mix(i + j);
@@ -144,22 +143,21 @@ __global__ __launch_bounds__(256) void adamw8_kernel(List<L> list) {
                 }
             }
             const uint32_t mw = encode4<false, STOCHASTIC>(mv, m_scale, um), vw = encode4<true, STOCHASTIC>(rv, v_scale, uv);
-            if (whole) {
+            if constexpr (whole.value) {
                 __builtin_nontemporal_store(mw, reinterpret_cast<u32_any*>(m + off));
                 __builtin_nontemporal_store(vw, reinterpret_cast<u32_any*>(v + off));
-                store4(pv, (P*)r.param + base + off);
-            } else if (off < count) {
-                store_codes(mw, m, off, count);
-                store_codes(vw, v, off, count);
-                for (uint32_t j = 0; j < 4 && off + j < count; ++j)
-                    if (!(k.flags & (o.b[j] ? kHoldB : kHold))) ((P*)r.param)[dense ? base + off + j : at(j, r.ld_param)] = (P)pv[j];
+                store4(pv, (P*)r.param + at.base + off);
+            } else {
+                store_codes(mw, m, off, at.count);
+                store_codes(vw, v, off, at.count);
+                for (uint32_t j = 0; j < 4 && off + j < at.count; ++j)
+                    if (!(k.flags & (o.b[j] ? kHoldB : kHold))) ((P*)r.param)[at(off + j, r.ld_param)] = (P)pv[j];
             }
-            if (off < count && (off & (GSX_MOMENT_RUN - 1)) == 0) { ms[run] = m_scale; vs[run] = v_scale; }
-            if (k.split || !dense) {
-                const uint32_t q = col + kChunk;
-                row += dense ? 0 : q / cols;
-                col = q % cols;
-            }
+            if (off < at.count && (off & (GSX_MOMENT_RUN - 1)) == 0) { ms[run] = m_scale; vs[run] = v_scale; }
+        };
+        for (; chunk < stop; ++chunk, at.next(kChunk)) {
+            if (at.whole) pass(std::true_type{});
+            else pass(std::false_type{});
         }
     });
 }
@@ -262,13 +260,14 @@ extern "C" int gsx_adamw8_step_multi(uint32_t count, const gsx_adamw_tensor* ten
     List<kFew> few;
     List<kMany> many;
     few.b = many.b = betas_of(beta1, beta2, eps, seed, control);
+    Corrections last = {};
     for (uint32_t types = 0; types < 9; ++types) {
         const uint32_t pd = types / 3, gd = types % 3;
         const int rc = launch_lists<Rec>(
             count, kChunk, kGrid, few.c, many.c,
             [&](uint32_t i, Rec* r, uint64_t* n) {
                 if (tensors[i].param_dtype != pd || tensors[i].grad_dtype != gd) return false;
-                *r = rec_of(tensors[i], i, few.b);
+                *r = rec_of(tensors[i], i, few.b, &last);
                 *n = r->n;
                 return true;
             },
