@@ -36,14 +36,14 @@ __global__ __launch_bounds__(256) void adamw_kernel(List<L> list) {
                     vv[j] = v[i];
                 }
             }
-            const Groups o = groups_of(k.split, at.col + off, at.cols);
+            uint32_t held = 0;
+            const Steps o = steps_of(k, at.mine, at.cols, whole.value ? nullptr : &held);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (k.flags & (o.b[j] ? kHoldB : kHold)) continue;
                 const float g1 = gv[j] * ctl.factor;
                 mv[j] = a.b1 * mv[j] + a.b1c * g1;
                 vv[j] = a.b2 * vv[j] + a.b2c * g1 * g1;
-                pv[j] = stepped(a, k, o.b[j], pv[j], mv[j], sqrtf(vv[j]));
+                pv[j] = stepped(a, k, o.lrwd[j], o.step[j], pv[j], mv[j], sqrtf(vv[j]));
             }
             if constexpr (whole.value) {
                 store4(mv, m + off);
@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(List<L> list) {
                 store4(pv, (P*)r.param + at.base + off);
             } else {
                 for (uint32_t j = 0; j < 4 && off + j < at.count; ++j) {
-                    if (k.flags & (o.b[j] ? kHoldB : kHold)) continue;
+                    if (held >> j & 1u) continue;
                     ((P*)r.param)[at(off + j, r.ld_param)] = (P)pv[j];
                     m[off + j] = mv[j];
                     v[off + j] = vv[j];
@@ -228,7 +228,7 @@ int check_adamw(uint32_t count, const gsx_adamw_tensor* tensors, double beta1, d
 }
 
 Betas betas_of(double beta1, double beta2, double eps, uint32_t seed, const double* control) {
-    return Betas{control, log(beta1), log(beta2), (float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, seed};
+    return Betas{control, log(beta1), log(beta2), (float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), std::max((float)eps, 0x1p-126f), seed};
 }
 
 Rec rec_of(const gsx_adamw_tensor& x, uint32_t ordinal, const Betas& b, Corrections* last) {

@@ -129,7 +129,7 @@ enum : uint32_t { kHold = 1, kHoldB = 2, kRows = 4 };   // kRows: parameter or g
 struct Betas {
     const double* control;
     double log_b1, log_b2;
-    float b1, b1c, b2, b2c, eps;
+    float b1, b1c, b2, b2c, eps;   // (eps at least 2^-126)
     uint32_t seed;
 };
 
@@ -164,51 +164,64 @@ GSX_DEV float second_moment(const Betas& a, float v, float g) {
     return a.b2 * v + a.b2c * g * g;
 }
 
-// Which of the four values that start `q` values behind the start of a row belong to the second column group.
-struct Groups { bool b[4]; };
-GSX_DEV Groups groups_of(uint32_t split, uint32_t q, uint32_t cols) {
-    Groups o = {{false, false, false, false}};
-    if (split) {
-        uint32_t c = q % cols;
+// The rates of a lane's four values, c the column of the first of them, and which of the values their group holds as they are.
+struct Steps { float lrwd[4], step[4]; };
+GSX_DEV Steps steps_of(const Rates& k, uint32_t c, uint32_t cols, uint32_t* held = nullptr) {
+    Steps o;
+    if (held) *held = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { o.lrwd[j] = k.lrwd; o.step[j] = k.step; }
+    if (k.split) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            o.b[j] = c >= split;
-            c = c + 1 == cols ? 0 : c + 1;
+            const bool b = c >= k.split;
+            o.lrwd[j] = b ? k.lrwd_b : k.lrwd;
+            o.step[j] = b ? k.step_b : k.step;
+            if (held) *held |= k.flags & (b ? kHoldB : kHold) ? 1u << j : 0u;
+            ++c;
+            c = std::min(c, c - cols);   // (c - cols wraps round to a large number while c is a column)
         }
+    } else if (held && (k.flags & kHold)) {
+        *held = 15u;
     }
     return o;
 }
 
-// One parameter's step, after its moments (root: sqrt(v)).
-GSX_DEV float stepped(const Betas& a, const Rates& k, bool b, float p, float m, float root) {
-    return p - (b ? k.lrwd_b : k.lrwd) * p - (b ? k.step_b : k.step) * m / (root * k.bc2 + a.eps);
+// One parameter's step, after its moments (root: sqrt(v)).  The denominator is at least eps, which is at least 2^-126 (betas_of): its reciprocal is the
+// hardware's (1 ulp).
+GSX_DEV float stepped(const Betas& a, const Rates& k, float lrwd, float step, float p, float m, float root) {
+    return p - lrwd * p - step * m * __builtin_amdgcn_rcpf(root * k.bc2 + a.eps);
 }
 
 // Where the values of a chunk lie.  Rows and columns are followed from chunk to chunk, and only where something goes by them.
 struct Place {
     const uint64_t n;
     const uint32_t cols;
-    const bool view, by_column;
+    const bool view, by_column, special;
     uint64_t base, row = 0;   // first value of the chunk, and its row (of a view)
     uint32_t col = 0, count;  // its column; values in the chunk
-    bool whole;               // all values of the chunk, one behind the other in all of the tensor's arrays
+    uint32_t mine = 0;        // column of the lane's first value (of four)
+    bool whole;               // a full chunk, its values one behind the other in all of the tensor's arrays, none of them held
     GSX_DEV Place(const Rec& r, uint32_t split, uint64_t first, uint32_t chunk)
-        : n(r.n), cols((uint32_t)r.cols), view(r.flags & kRows), by_column(split || view), base(first) {
+        : n(r.n), cols((uint32_t)r.cols), view(r.flags & kRows), by_column(split || view), special(r.flags != 0), base(first) {
         if (by_column) {
             row = base / r.cols;
             col = (uint32_t)(base - row * r.cols);
+            mine = (col + threadIdx.x * 4u) % cols;
         }
         size(chunk);
     }
     GSX_DEV void size(uint32_t chunk) {
         count = (uint32_t)std::min<uint64_t>(n - base, chunk);
-        whole = !view && count == chunk;
+        whole = !special && count == chunk;
     }
     GSX_DEV void next(uint32_t chunk) {
         base += chunk;
         if (by_column) {
             const uint32_t q = col + chunk, dr = q / cols;
             row += dr;
+            mine += q - dr * cols >= col ? q - dr * cols - col : q - dr * cols + cols - col;   // (the step from column to column, less than cols)
+            mine = std::min(mine, mine - cols);
             col = q - dr * cols;
         }
         size(chunk);   // (behind the last chunk: not used)

@@ -6,6 +6,7 @@ namespace optim {
 
 constexpr uint32_t kChunk = 1024;   // values of one pass of a workgroup: four of each lane, 32 lanes to a run
 constexpr uint32_t kGrid = 16384;   // workgroups of a launch at most
+constexpr uint32_t kInfinity = 0x7F800000u;
 constexpr float kCodeTop = 448.0f, kScaleFloor = 0x1p-120f, kCodeMin = 0x1p-9f;
 static_assert(GSX_MOMENT_RUN == 128, "the exchanges below are among 32 lanes of four values");
 
@@ -15,31 +16,63 @@ GSX_DEV uint32_t mix(uint32_t x) {
     return x ^ (x >> 16);
 }
 
-template <int C> GSX_DEV float dpp_max(float x) {
-    return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), C, 0xF, 0xF, true)));
+// Square roots to the last bit: x times the hardware's reciprocal root (1 ulp), corrected by what that leaves of x.  For 2^-96 and up, and zero; where a wave has
+// others (smaller: the remainder would be subnormal; infinities, NaN) the library's root, which takes twice the instructions.
+GSX_DEV f32x4 roots(f32x4 x) {
+    uint32_t low = 0xFFFFFFFFu, high = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        low = std::min(low, __float_as_uint(x[j]) - 1u);   // (zero becomes the largest)
+        high = std::max(high, __float_as_uint(x[j]));
+    }
+    f32x4 r;
+    if (__any(low < 0x0F800000u - 1u || high >= kInfinity)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = sqrtf(x[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float y = __builtin_amdgcn_rsqf(fmaxf(x[j], 0x1p-126f)), s = x[j] * y;
+            r[j] = fmaf(fmaf(-s, s, x[j]), 0.5f * y, s);
+        }
+    }
+    return r;
 }
-// Largest of the 32 lanes that hold a run (4 values each), in all of them; every lane of the wave takes part.
-GSX_DEV float run_max(float x) {
+
+// Largest of the 32 lanes that hold a run (4 values each), in all of them; every lane of the wave takes part.  Floats from zero up, compared as whole numbers.
+template <int C> GSX_DEV uint32_t dpp_max(uint32_t x) {
+    return std::max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, C, 0xF, 0xF, true));
+}
+GSX_DEV uint32_t run_max(uint32_t x) {
     x = dpp_max<0xB1>(x);    // neighbours
     x = dpp_max<0x4E>(x);    // pairs of a quad
     x = dpp_max<0x141>(x);   // halves of eight
     x = dpp_max<0x140>(x);   // halves of a row of 16
-    return fmaxf(x, __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(x), 0x401F)));   // rows of a run
+    return std::max(x, (uint32_t)__builtin_amdgcn_ds_swizzle((int)x, 0x401F));   // rows of a run
 }
-GSX_DEV float top_of(f32x4 x) {
-    const float top = run_max(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));   // (fmaxf passes over NaN)
-    if (__any(isinf(top))) {   // a run with infinities: the largest of the finite values
-        float f = 0.0f;
-        for (int j = 0; j < 4; ++j) f = fmaxf(f, isinf(x[j]) ? 0.0f : fabsf(x[j]));
-        return run_max(f);
+GSX_DEV uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+GSX_DEV uint32_t top_of(f32x4 x) { return std::max(std::max(std::max(magnitude(x.x), magnitude(x.y)), magnitude(x.z)), magnitude(x.w)); }
+GSX_DEV uint32_t finite_top_of(f32x4 x) {
+    uint32_t f = 0;
+    for (int j = 0; j < 4; ++j) f = std::max(f, magnitude(x[j]) < kInfinity ? magnitude(x[j]) : 0u);
+    return f;
+}
+GSX_DEV float scale_of(uint32_t top) { return fmaxf(__uint_as_float(top) * (1.0f / kCodeTop), kScaleFloor); }
+// The scales of a run's two moments: of their largest finite values.
+GSX_DEV void scales_of(f32x4 m, f32x4 r, float* m_scale, float* r_scale) {
+    uint32_t mt = run_max(top_of(m)), rt = run_max(top_of(r));
+    if (__any(std::max(mt, rt) >= kInfinity)) {   // infinities or NaN among them
+        mt = run_max(finite_top_of(m));
+        rt = run_max(finite_top_of(r));
     }
-    return top;
+    *m_scale = scale_of(mt);
+    *r_scale = scale_of(rt);
 }
-GSX_DEV float scale_of(float top) { return fmaxf(top * (1.0f / kCodeTop), kScaleFloor); }
 
-// x / scale to the last bit, by the reciprocal that the four share: the quotient's estimate, what it leaves of x (exact), and the correction that this gives.
+// x / scale to the last bit, by the reciprocal that the four share (the hardware's, 1 ulp: a scale is neither below 2^-120 nor above 2^120): the quotient's estimate,
+// what it leaves of x, and the correction that this gives.
 GSX_DEV f32x4 over(f32x4 x, float scale) {
-    const float inv = 1.0f / scale;
+    const float inv = __builtin_amdgcn_rcpf(scale);
     f32x4 y;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -122,16 +155,30 @@ __global__ __launch_bounds__(256) void adamw8_kernel(List<L> list) {
                 rv = decode4(vw, vs[here]);
             }
             // (from here on every lane, also those behind the end: the lanes of a run exchange their largest values)
-            const Groups o = groups_of(k.split, at.col + off, at.cols);
+            uint32_t held = 0;
+            const Steps o = steps_of(k, at.mine, at.cols, whole.value ? nullptr : &held);
+            f32x4 m1, r1;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (k.flags & (o.b[j] ? kHoldB : kHold)) continue;
-                const float g1 = gv[j] * ctl.factor;
-                mv[j] = first_moment(a, mv[j], g1);
-                rv[j] = sqrtf(second_moment(a, rv[j] * rv[j], g1));
-                pv[j] = stepped(a, k, o.b[j], pv[j], mv[j], rv[j]);
+                gv[j] *= ctl.factor;
+                m1[j] = first_moment(a, mv[j], gv[j]);
+                r1[j] = second_moment(a, rv[j] * rv[j], gv[j]);
             }
-            const float m_scale = scale_of(top_of(mv)), v_scale = scale_of(top_of(rv));
+            r1 = roots(r1);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pv[j] = stepped(a, k, o.lrwd[j], o.step[j], pv[j], m1[j], r1[j]);
+            if constexpr (whole.value) {
+                mv = m1;
+                rv = r1;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    mv[j] = held >> j & 1u ? mv[j] : m1[j];
+                    rv[j] = held >> j & 1u ? rv[j] : r1[j];
+                }
+            }
+            float m_scale, v_scale;
+            scales_of(mv, rv, &m_scale, &v_scale);
             uint32_t um[4], uv[4];
             if (STOCHASTIC) {
                 const uint32_t i = (uint32_t)at.base + key + 0x61C8864Fu * (uint32_t)(at.base >> 32) + off;
@@ -139,7 +186,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(List<L> list) {
                 for (uint32_t j = 0; j < 4; ++j) {
                     const uint32_t w = mix(i + j);
                     um[j] = w & 0xFFFF0000u;
-                    uv[j] = w << 16;
+                    uv[j] = __builtin_amdgcn_perm(w, 0u, 0x05040C0Cu);   // w << 16 (as a shift it would become a third product)
                 }
             }
             const uint32_t mw = encode4<false, STOCHASTIC>(mv, m_scale, um), vw = encode4<true, STOCHASTIC>(rv, v_scale, uv);
@@ -151,7 +198,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(List<L> list) {
                 store_codes(mw, m, off, at.count);
                 store_codes(vw, v, off, at.count);
                 for (uint32_t j = 0; j < 4 && off + j < at.count; ++j)
-                    if (!(k.flags & (o.b[j] ? kHoldB : kHold))) ((P*)r.param)[at(off + j, r.ld_param)] = (P)pv[j];
+                    if (!(held >> j & 1u)) ((P*)r.param)[at(off + j, r.ld_param)] = (P)pv[j];
             }
             if (off < at.count && (off & (GSX_MOMENT_RUN - 1)) == 0) { ms[run] = m_scale; vs[run] = v_scale; }
         };
@@ -231,7 +278,8 @@ template <uint32_t L> __global__ __launch_bounds__(256) void select_rows_kernel(
                     mv[j] = off + j < count ? lds[0][off + j] : 0.0f;
                     rv[j] = off + j < count ? lds[1][off + j] : 0.0f;
                 }
-                const float m_scale = scale_of(top_of(mv)), v_scale = scale_of(top_of(rv));
+                float m_scale, v_scale;
+                scales_of(mv, rv, &m_scale, &v_scale);
                 if (off >= count) continue;
                 const uint32_t mw = encode4<false, false>(mv, m_scale, nullptr), vw = encode4<true, false>(rv, v_scale, nullptr);
                 if (off + 4 <= count) {
