@@ -80,9 +80,9 @@ inline bool count_of(uint64_t rows, uint64_t cols, uint64_t* n) {
 }
 
 // Gathers tensors and launches them: item(i, &rec, &values) is false for a tensor that does not belong to this launch; launch(list) for every full list.  `few` and
-// `many` are the two argument blocks (host), `grid` the most workgroups of a launch.
-template <class R, class Few, class Many, class Item, class Launch>
-int launch_lists(uint32_t count, uint32_t chunk, uint32_t grid, Few& few, Many& many, Item item, Launch launch) {
+// `many` are the two argument blocks (host); per(chunks): how many of them a workgroup takes.
+template <class R, class Few, class Many, class Per, class Item, class Launch>
+int launch_lists(uint32_t count, uint32_t chunk, Per per, Few& few, Many& many, Item item, Launch launch) {
     uint32_t i = 0;
     while (i < count) {
         uint32_t k = 0;
@@ -92,17 +92,23 @@ int launch_lists(uint32_t count, uint32_t chunk, uint32_t grid, Few& few, Many& 
             uint64_t n = 0;
             if (!item(i, &rec, &n) || n == 0) continue;
             if (k == kMany || (k != 0 && chunks + chunks_of(n, chunk) > kMostChunks)) break;
-            if (k < kFew) few.rec[k] = rec, few.begin[k] = (uint32_t)chunks;
-            many.rec[k] = rec;
-            many.begin[k++] = (uint32_t)chunks;
+            if (k < kFew) {
+                few.rec[k] = rec;
+                few.begin[k] = (uint32_t)chunks;
+            } else {
+                if (k == kFew) { std::copy_n(few.rec, kFew, many.rec); std::copy_n(few.begin, kFew, many.begin); }
+                many.rec[k] = rec;
+                many.begin[k] = (uint32_t)chunks;
+            }
+            ++k;
             chunks += chunks_of(n, chunk);
         }
         if (k == 0) break;
         auto finish = [&](auto& a, uint32_t room) {
             for (uint32_t j = k; j <= room; ++j) a.begin[j] = 0xFFFFFFFFu;
             a.chunks = (uint32_t)chunks;
-            a.per = (uint32_t)((chunks + grid - 1) / grid);
-            return launch(a, (uint32_t)((chunks + a.per - 1) / a.per));
+            a.per = per((uint32_t)chunks);
+            return launch(a, (a.chunks + a.per - 1) / a.per);
         };
         const int rc = k <= kFew ? finish(few, kFew) : finish(many, kMany);
         if (rc != GSX_OK) return rc;
@@ -133,8 +139,16 @@ struct Betas {
     uint32_t seed;
 };
 
-// What the control block says, and the bias corrections of its step: 1 - beta^t = -expm1(t log beta), whose relative error is that of the product (2^-24),
-// where 1 - pow() would lose beta's own rounding (0.999 in 32 bits: 3e-5 of 1 - beta).
+// 1 - exp(x), x <= 0, to a few 2^-24 of itself: the series where it is small, where 1 - exp(x) would lose its leading digits (beta2 = 0.999, first step: 1e-4 of it).
+// A third of the library's expm1f in instructions; every workgroup computes it.
+GSX_DEV float one_minus_exp(float x) {
+    float s = 1.0f / 40320.0f;   // (1 + x/2 + x^2/6 + ...: what is cut is below x^8 / 9!, 2^-26 at -1/2)
+    s = fmaf(s, x, 1.0f / 5040.0f); s = fmaf(s, x, 1.0f / 720.0f); s = fmaf(s, x, 1.0f / 120.0f);
+    s = fmaf(s, x, 1.0f / 24.0f); s = fmaf(s, x, 1.0f / 6.0f); s = fmaf(s, x, 0.5f); s = fmaf(s, x, 1.0f);
+    return x > -0.5f ? -x * s : 1.0f - __builtin_amdgcn_exp2f(x * 1.44269504f);
+}
+
+// What the control block says, and the bias corrections of its step.  1 - beta^t = 1 - exp(t log beta), the product in 64 bits.
 struct Control { bool skip; float factor, bc1, bc2; uint32_t step; };
 GSX_DEV Control control_of(const Betas& a) {
     Control c = {false, 1.0f, 0.0f, 0.0f, 0u};
@@ -142,8 +156,8 @@ GSX_DEV Control control_of(const Betas& a) {
     c.skip = a.control[2] != 0.0;
     c.factor = (float)a.control[1];
     c.step = std::max((uint32_t)a.control[3], 1u);   // (a block that no norm has advanced: the first step)
-    c.bc1 = 1.0f / -expm1f((float)(a.log_b1 * (double)c.step));
-    c.bc2 = 1.0f / sqrtf(-expm1f((float)(a.log_b2 * (double)c.step)));
+    c.bc1 = __builtin_amdgcn_rcpf(one_minus_exp((float)(a.log_b1 * (double)c.step)));
+    c.bc2 = __builtin_amdgcn_rsqf(one_minus_exp((float)(a.log_b2 * (double)c.step)));
     return c;
 }
 
@@ -202,13 +216,15 @@ struct Place {
     uint32_t col = 0, count;  // its column; values in the chunk
     uint32_t mine = 0;        // column of the lane's first value (of four)
     bool whole;               // a full chunk, its values one behind the other in all of the tensor's arrays, none of them held
-    GSX_DEV Place(const Rec& r, uint32_t split, uint64_t first, uint32_t chunk)
-        : n(r.n), cols((uint32_t)r.cols), view(r.flags & kRows), by_column(split || view), special(r.flags != 0), base(first) {
-        if (by_column) {
+    GSX_DEV Place(const Rec& r, uint32_t split, uint32_t index, uint32_t chunk)
+        : n(r.n), cols((uint32_t)r.cols), view(r.flags & kRows), by_column(split || view), special(r.flags != 0), base((uint64_t)index * chunk) {
+        if (view || (split && cols > 0xFFFFu)) {
             row = base / r.cols;
             col = (uint32_t)(base - row * r.cols);
-            mine = (col + threadIdx.x * 4u) % cols;
+        } else if (split) {   // (the same without a quotient of 64 bits, which would be a fifth of the instructions of a pass)
+            col = (index % cols) * (chunk % cols) % cols;
         }
+        if (by_column) mine = (col + threadIdx.x * 4u) % cols;
         size(chunk);
     }
     GSX_DEV void size(uint32_t chunk) {
@@ -233,6 +249,13 @@ struct Place {
         return (row + dr) * ld + (q - dr * cols);
     }
 };
+
+// The pairs of parameter and gradient types among the tensors: bit 3 * param_dtype + grad_dtype.
+inline uint32_t types_of(uint32_t count, const gsx_adamw_tensor* tensors) {
+    uint32_t mask = 0;
+    for (uint32_t i = 0; i < count; ++i) mask |= 1u << (3 * tensors[i].param_dtype + tensors[i].grad_dtype);
+    return mask;
+}
 
 struct Corrections { uint64_t step; float bc1, bc2; };
 int check_adamw(uint32_t count, const gsx_adamw_tensor* tensors, double beta1, double beta2, double eps, bool eight, const double* control);

@@ -5,7 +5,9 @@ namespace gsx {
 namespace optim {
 
 constexpr uint32_t kChunk = 1024;   // values of one pass of a workgroup: four of each lane, 32 lanes to a run
-constexpr uint32_t kGrid = 16384;   // workgroups of a launch at most
+// Chunks of a workgroup: two in a row share its start, where there are workgroups enough to fill the card either way; more spread what is in flight too far
+// (5 M splats: 786 us with two, 838 with one, 840 with eight; 1 M: 164, 183, 173).
+inline uint32_t per_of(uint32_t chunks) { return chunks >= 4096 ? 2 : 1; }
 constexpr uint32_t kInfinity = 0x7F800000u;
 constexpr float kCodeTop = 448.0f, kScaleFloor = 0x1p-120f, kCodeMin = 0x1p-9f;
 static_assert(GSX_MOMENT_RUN == 128, "the exchanges below are among 32 lanes of four values");
@@ -131,7 +133,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(List<L> list) {
         const Rates k = rates_of(r, ctl);
         const uint32_t off = threadIdx.x * 4u, run = off / GSX_MOMENT_RUN;
         const uint32_t key = STOCHASTIC ? mix(mix(a.seed + 0x9E3779B9u * (r.step ? r.step : ctl.step)) + 0xC2A6F0B5u * r.ordinal) : 0u;
-        Place at(r, k.split, (uint64_t)chunk * kChunk, kChunk);
+        Place at(r, k.split, chunk, kChunk);
         auto pass = [&](auto whole) {   // (compiled twice: the ends of tensors and the views stay out of the way of the whole chunks)
             uint8_t* m = (uint8_t*)r.m + at.base; uint8_t* v = (uint8_t*)r.v + at.base;
             float* ms = r.m_scale + at.base / GSX_MOMENT_RUN; float* vs = r.v_scale + at.base / GSX_MOMENT_RUN;
@@ -217,66 +219,106 @@ template <uint32_t L> struct SelectList {
     uint64_t rows_in, rows_out;
 };
 
-constexpr uint32_t kSelect = 2048;   // values of one pass of a workgroup
+constexpr uint32_t kSelect = 2048;   // values of one pass of a workgroup (1 M splats 171 us, 181 with 4 096: less LDS, more workgroups at once)
 
-// A chunk of the new moments is gathered into LDS in pieces of up to four values of one row (an index, two codes words and two scales a piece, whatever the rows' length and
-// the places where old and new runs begin), then coded from there like the update's.
-template <uint32_t L> __global__ __launch_bounds__(256) void select_rows_kernel(SelectList<L> a) {
-    __shared__ float lds[2][kSelect];
-    walk(a.c, [&](const SelectRec& r, uint32_t chunk, uint32_t stop) {
-        const uint32_t cols = (uint32_t)r.cols, pieces = (cols + 3) / 4;
-        const uint64_t n = a.rows_out * r.cols, n_in = a.rows_in * r.cols;
-        for (; chunk < stop; ++chunk) {
-            const uint64_t base = (uint64_t)chunk * kSelect, row0 = base / r.cols;
-            const uint32_t count = (uint32_t)std::min<uint64_t>(n - base, kSelect);
-            const uint32_t col0 = (uint32_t)(base - row0 * r.cols);
-            const uint32_t first = col0 / 4, items = (uint32_t)(((uint64_t)col0 + count + cols - 1) / cols) * pieces;   // (of all rows that the chunk touches)
-            __syncthreads();
-            for (uint32_t i = first + threadIdx.x; i < items; i += 256u) {
-                const uint32_t dr = i / pieces, c = (i - dr * pieces) * 4u, len = std::min(cols - c, 4u);
-                const int64_t to = (int64_t)dr * cols + c - col0;   // where in the chunk; a piece may start before it and end behind it
-                if (to >= (int64_t)count) break;
-                const int64_t src = a.index[row0 + dr];
-                f32x4 mv = {0, 0, 0, 0}, rv = {0, 0, 0, 0};
-                if (src >= 0 && (uint64_t)src < a.rows_in) {
-                    const uint64_t at = (uint64_t)src * cols + c;
-                    const uint64_t s0 = at / GSX_MOMENT_RUN, s1 = (at + len - 1) / GSX_MOMENT_RUN;
-                    uint32_t mw, vw;
-                    if (at + 4 <= n_in) {
-                        mw = *reinterpret_cast<const u32_any*>(r.m + at);
-                        vw = *reinterpret_cast<const u32_any*>(r.v + at);
-                    } else {
-                        mw = load_codes(r.m + at, 0, len);
-                        vw = load_codes(r.v + at, 0, len);
-                    }
-                    mv = decode4(mw, 1.0f);
-                    rv = decode4(vw, 1.0f);
-                    const float ms = r.ms[s0], vs = r.vs[s0];
-                    float ms1 = ms, vs1 = vs;
-                    if (s1 != s0) { ms1 = r.ms[s1]; vs1 = r.vs[s1]; }
-                    const uint32_t left = GSX_MOMENT_RUN - (uint32_t)(at % GSX_MOMENT_RUN);   // values up to the next run
+// n / d for n < 2^22, d < 2^22 (the quotient's estimate is off by one at most).
+GSX_DEV uint32_t small_div(uint32_t n, uint32_t d, float rcp) {
+    uint32_t q = (uint32_t)((float)n * rcp);
+    q -= q * d > n ? 1u : 0u;
+    return n - q * d >= d ? q + 1u : q;
+}
+
+// A chunk of the new moments is gathered into LDS in pieces of one row (an index, two loads of codes and two scales a piece, whatever the rows' length and the places where
+// old and new runs begin), then coded from there like the update's.  A piece has W = 16 values where the rows' length is a multiple of 16 (the SH coefficients of degree
+// 3: 48), then no piece crosses the end of a run either; else up to four.
+// What bounds it: two dependent loads from random places, of which a row of 48 bytes costs 121 of the memory's (455 MB for 1 M splats, 122 MB of codes).
+template <uint32_t W> struct Codes { uint32_t m[W / 4], v[W / 4]; };
+template <uint32_t W, uint32_t BATCH>
+GSX_DEV void gather(const SelectRec& r, const int64_t* __restrict__ index, uint64_t rows_in, uint64_t row0, uint32_t col0, uint32_t count, float (*lds)[kSelect]) {
+    const uint32_t cols = (uint32_t)r.cols, pieces = (cols + W - 1) / W, last = col0 + count - 1u;
+    const uint64_t n_in = rows_in * r.cols;
+    const uint32_t items = last / cols * pieces + last % cols / W + 1u;   // pieces from the start of the first row to the last value
+    const bool small = items < (1u << 22) && pieces < (1u << 22);
+    const float rcp = 1.0f / (float)pieces;
+    for (uint32_t i = col0 / W + threadIdx.x; i < items; i += 256u * BATCH) {
+        uint32_t c[BATCH], len[BATCH], left[BATCH];
+        int32_t to[BATCH];   // where in the chunk a piece goes; the first may start before it and the last end behind it
+        int64_t src[BATCH];
+        Codes<W> w[BATCH];
+        float m0[BATCH], v0[BATCH], m1[BATCH], v1[BATCH];
 #pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) {
-                        mv[j] *= j < left ? ms : ms1;
-                        rv[j] *= j < left ? vs : vs1;
-                    }
+        for (uint32_t b = 0; b < BATCH; ++b) {
+            const uint32_t item = std::min(i + 256u * b, items - 1u), dr = small ? small_div(item, pieces, rcp) : item / pieces;
+            c[b] = (item - dr * pieces) * W;
+            len[b] = std::min(cols - c[b], W);
+            to[b] = (int32_t)(dr * cols + c[b] - col0);
+            src[b] = index[row0 + dr];
+        }
+#pragma unroll
+        for (uint32_t b = 0; b < BATCH; ++b) {
+            w[b] = Codes<W>{};
+            m0[b] = v0[b] = m1[b] = v1[b] = 0.0f;
+            left[b] = W;
+            if (src[b] < 0 || (uint64_t)src[b] >= rows_in) continue;
+            const uint64_t at = (uint64_t)src[b] * cols + c[b], run = at / GSX_MOMENT_RUN;
+            if (W == 16 || at + 4 <= n_in) {
+#pragma unroll
+                for (uint32_t k = 0; k < W / 4; ++k) {
+                    w[b].m[k] = reinterpret_cast<const u32_any*>(r.m + at)[k];
+                    w[b].v[k] = reinterpret_cast<const u32_any*>(r.v + at)[k];
                 }
+            } else {
+                w[b].m[0] = load_codes(r.m + at, 0, len[b]);
+                w[b].v[0] = load_codes(r.v + at, 0, len[b]);
+            }
+            m0[b] = r.ms[run];
+            v0[b] = r.vs[run];
+            if (W == 4) {
+                left[b] = GSX_MOMENT_RUN - (uint32_t)(at % GSX_MOMENT_RUN);   // values up to the next run
+                if (left[b] < len[b]) { m1[b] = r.ms[run + 1]; v1[b] = r.vs[run + 1]; }
+            }
+        }
 #pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    if (j < len && to + j >= 0 && to + j < (int64_t)count) {
-                        lds[0][to + j] = mv[j];
-                        lds[1][to + j] = rv[j];
-                    }
+        for (uint32_t b = 0; b < BATCH; ++b) {
+            if (i + 256u * b >= items) continue;
+            if (W == 16) {
+#pragma unroll
+                for (uint32_t k = 0; k < W / 4; ++k) {
+                    *reinterpret_cast<f32x4*>(&lds[0][to[b] + 4 * k]) = decode4(w[b].m[k], m0[b]);
+                    *reinterpret_cast<f32x4*>(&lds[1][to[b] + 4 * k]) = decode4(w[b].v[k], v0[b]);
+                }
+                continue;
+            }
+            const f32x4 mv = decode4(w[b].m[0], 1.0f), rv = decode4(w[b].v[0], 1.0f);
+#pragma unroll
+            for (int32_t j = 0; j < 4; ++j) {
+                if (j < (int32_t)len[b] && to[b] + j >= 0 && to[b] + j < (int32_t)count) {
+                    lds[0][to[b] + j] = mv[j] * ((uint32_t)j < left[b] ? m0[b] : m1[b]);
+                    lds[1][to[b] + j] = rv[j] * ((uint32_t)j < left[b] ? v0[b] : v1[b]);
                 }
             }
+        }
+    }
+}
+
+template <uint32_t L> __global__ __launch_bounds__(256) void select_rows_kernel(SelectList<L> a) {
+    __shared__ __align__(16) float lds[2][kSelect];
+    walk(a.c, [&](const SelectRec& r, uint32_t chunk, uint32_t stop) {
+        const uint64_t n = a.rows_out * r.cols;
+        for (; chunk < stop; ++chunk) {
+            const uint64_t base = (uint64_t)chunk * kSelect, row0 = base >> 32 ? base / r.cols : (uint32_t)base / (uint32_t)r.cols;
+            const uint32_t count = (uint32_t)std::min<uint64_t>(n - base, kSelect), col0 = (uint32_t)(base - row0 * r.cols);
+            __syncthreads();
+            if (r.cols % 16 == 0) gather<16, 1>(r, a.index, a.rows_in, row0, col0, count, lds);
+            else gather<4, 3>(r, a.index, a.rows_in, row0, col0, count, lds);
             __syncthreads();
             for (uint32_t pass = 0; pass < kSelect; pass += 1024u) {   // (the same number of passes for every lane: the runs' lanes exchange their largest values)
                 const uint32_t off = pass + threadIdx.x * 4u;
-                f32x4 mv, rv;
+                f32x4 mv = *reinterpret_cast<const f32x4*>(&lds[0][off]), rv = *reinterpret_cast<const f32x4*>(&lds[1][off]);
 #pragma unroll
                 for (uint32_t j = 0; j < 4; ++j) {
-                    mv[j] = off + j < count ? lds[0][off + j] : 0.0f;
-                    rv[j] = off + j < count ? lds[1][off + j] : 0.0f;
+                    mv[j] = off + j < count ? mv[j] : 0.0f;
+                    rv[j] = off + j < count ? rv[j] : 0.0f;
                 }
                 float m_scale, v_scale;
                 scales_of(mv, rv, &m_scale, &v_scale);
@@ -309,10 +351,12 @@ extern "C" int gsx_adamw8_step_multi(uint32_t count, const gsx_adamw_tensor* ten
     List<kMany> many;
     few.b = many.b = betas_of(beta1, beta2, eps, seed, control);
     Corrections last = {};
+    const uint32_t mask = types_of(count, tensors);
     for (uint32_t types = 0; types < 9; ++types) {
+        if (!(mask >> types & 1u)) continue;
         const uint32_t pd = types / 3, gd = types % 3;
         const int rc = launch_lists<Rec>(
-            count, kChunk, kGrid, few.c, many.c,
+            count, kChunk, per_of, few.c, many.c,
             [&](uint32_t i, Rec* r, uint64_t* n) {
                 if (tensors[i].param_dtype != pd || tensors[i].grad_dtype != gd) return false;
                 *r = rec_of(tensors[i], i, few.b, &last);
@@ -358,7 +402,7 @@ extern "C" int gsx_adamw8_select_rows(uint32_t count, const gsx_moments8* tensor
     few.rows_in = many.rows_in = rows_in;
     few.rows_out = many.rows_out = rows_out;
     return launch_lists<SelectRec>(
-        count, kSelect, kGrid, few.c, many.c,
+        count, kSelect, [](uint32_t) { return 1u; }, few.c, many.c,
         [&](uint32_t i, SelectRec* r, uint64_t* n) {
             const gsx_moments8& x = tensors[i];
             *r = SelectRec{(const uint8_t*)x.avg_in, (const uint8_t*)x.rms_in, x.avg_scale_in, x.rms_scale_in, (uint8_t*)x.avg_out, (uint8_t*)x.rms_out,

@@ -1261,8 +1261,7 @@ void adamw_multi(const char* op, const TensorList& params, const TensorList& exp
         const auto state = eight ? at::kFloat8_e4m3fn : at::kFloat;
         TORCH_CHECK(m.scalar_type() == state && v.scalar_type() == state && m.is_contiguous() && v.is_contiguous(), op, ": the moments of parameter ", i,
                     " are contiguous ", state, " tensors");
-        gsx_adamw_tensor& x = list[i];
-        x = gsx_adamw_tensor{};
+        gsx_adamw_tensor& x = list[i];   // (all zero)
         x.param_dtype = optim_dtype(p, op, "parameter", i);
         x.grad_dtype = optim_dtype(g, op, "gradient", i);
         uint64_t rp, cp, rg, cg;
