@@ -209,6 +209,9 @@ uint32_t norm_blocks(uint32_t count, const gsx_grad_tensor* tensors) {
     return std::max(sum, 1u);
 }
 
+// Room for the sums of all workgroups: three types, each in launches of up to kMany tensors.
+size_t norm_bytes(uint32_t count) { return ((size_t)count / kMany + 3) * kNormGrid * sizeof(double); }
+
 // ---- what both AdamW entry points check and prepare -----------------------------------------------------------------------------------------------------
 int check_adamw(uint32_t count, const gsx_adamw_tensor* tensors, double beta1, double beta2, double eps, bool eight, const double* control) {
     if (count == 0) return GSX_OK;
@@ -292,8 +295,7 @@ extern "C" int gsx_adamw_step_multi(uint32_t count, const gsx_adamw_tensor* tens
 }
 
 extern "C" size_t gsx_grad_norm_multi_workspace_bytes(uint32_t count, const gsx_grad_tensor* tensors) {
-    if (check_grads(count, tensors) != GSX_OK) return 0;
-    return ((size_t)count / kMany + 3) * kNormGrid * sizeof(double);   // (three types, each in launches of up to kMany tensors)
+    return check_grads(count, tensors) == GSX_OK ? norm_bytes(count) : 0;
 }
 
 extern "C" int gsx_grad_norm_multi(uint32_t count, const gsx_grad_tensor* tensors, double max_norm, double* control, void* workspace,
@@ -303,7 +305,7 @@ extern "C" int gsx_grad_norm_multi(uint32_t count, const gsx_grad_tensor* tensor
     if (!(max_norm > 0.0)) return invalid("grad_norm_multi: max_norm is positive (infinite for no clipping)");
     if (control == nullptr || workspace == nullptr) return invalid("grad_norm_multi: null control block or workspace");
     const uint32_t blocks = norm_blocks(count, tensors);
-    if (workspace_bytes < blocks * sizeof(double)) { set_error("grad_norm_multi: workspace too small"); return GSX_ERR_WORKSPACE_TOO_SMALL; }
+    if (workspace_bytes < std::max(norm_bytes(count), blocks * sizeof(double))) { set_error("grad_norm_multi: workspace too small"); return GSX_ERR_WORKSPACE_TOO_SMALL; }
     uint64_t bytes = 0;
     for (uint32_t i = 0; i < count; ++i) bytes += tensors[i].rows * tensors[i].cols * (tensors[i].dtype == GSX_DTYPE_F32 ? 4 : 2);
     const NormEnd end = {(double*)workspace, control, max_norm, blocks};

@@ -11,7 +11,10 @@ advances; with `skip_sh_steps` (a compile-time switch upstream, default off) it 
 until iteration 25000.
 
 Groups address the model's tensors by name at step time, so a densification strategy may replace them by longer ones
-(`extend_state`) or reset the moments of relocated Gaussians (`reset_state`), as strategies/mcmc.cpp:85-112,252-330 do."""
+(`extend_state`) or reset the moments of relocated Gaussians (`reset_state`), as strategies/mcmc.cpp:85-112,252-330 do.
+
+FusedAdamW is AdamW in the same place: decoupled decay, a clip by the global gradient norm, moments in 32 or in 8 bits
+(csrc/gsx_adamw.hip, gsx_adamw8.hip)."""
 import math
 
 import torch
@@ -20,6 +23,14 @@ from . import ops
 
 GROUPS = ("means", "sh0", "shN", "scaling", "rotation", "opacity")
 _ATTR = {"means": "means", "sh0": "sh", "shN": "sh", "scaling": "scaling_raw", "rotation": "rotation_raw", "opacity": "opacity_raw"}
+
+
+def splat_rates(means_lr, shs_lr, scaling_lr, rotation_lr, opacity_lr, scene_scale):
+    """Learning rate of each group (FusedAdam.for_splat_data says how they are formed)."""
+    import numpy as np
+    f = np.float32
+    return {"means": float(f(means_lr) * f(scene_scale)), "sh0": float(f(shs_lr)), "shN": float(f(shs_lr) / f(20.0)),
+            "scaling": float(f(scaling_lr)), "rotation": float(f(rotation_lr)), "opacity": float(f(opacity_lr))}
 
 
 class FusedAdam:
@@ -38,10 +49,7 @@ class FusedAdam:
         learning rates are formed in fp32 before they are widened to the optimizer's double (`_params->means_lr * get_scene_scale()`,
         `_params->shs_lr / 20.f`): the same here — 0.00016f is 0.00015999999595806003, not 0.00016, and the scheduler multiplies that double every
         iteration (found by running the reference's own mcmc.cpp next to this class: tests/test_gpu_reference_strategy.py)."""
-        import numpy as np
-        f = np.float32
-        return FusedAdam(model, {"means": float(f(means_lr) * f(scene_scale)), "sh0": float(f(shs_lr)), "shN": float(f(shs_lr) / f(20.0)),
-                                 "scaling": float(f(scaling_lr)), "rotation": float(f(rotation_lr)), "opacity": float(f(opacity_lr))}, **kw)
+        return FusedAdam(model, splat_rates(means_lr, shs_lr, scaling_lr, rotation_lr, opacity_lr, scene_scale), **kw)
 
     # ---- state ---------------------------------------------------------------------------------------------------------
     def _param(self, name):
@@ -179,6 +187,147 @@ class FusedAdam:
                     p.grad = None
                 else:
                     p.grad.zero_()
+
+
+def decode_moment(codes, scale):
+    """The values that an 8-bit moment stands for: float32, of the codes' shape."""
+    run = ops.MOMENT_RUN
+    return (codes.float().reshape(-1) * scale.repeat_interleave(run)[:codes.numel()]).reshape(codes.shape)
+
+
+class FusedAdamW(FusedAdam):
+    """AdamW on the same six groups (ops.adamw_step_multi / adamw8_step_multi: the whole model in one launch), in FusedAdam's place: MCMC(make_optimizer=...),
+    Trainer(optimizer="adamw" | "adamw8").  What it adds:
+
+    weight_decay   decoupled decay of the groups that the dict names.  The groups hold raw parameters: decay pulls opacities towards 1/2, scales towards 1,
+                   positions towards the origin; of the splat groups shN (the view-dependent colour) is the one that usually wants it.
+    moments=8      both moments as float8_e4m3fn numbers with a scale for every 128: 2 bytes a parameter in place of 8 (1 M Gaussians of SH degree 3: 0.12 in place of 0.47 GB,
+                   and the step moves 16 bytes a parameter in place of 28).  Rounded stochastically, from `seed` and the step (seed=None: to nearest, under which the second
+                   moment comes to rest: include/gsx_optim.h).
+    max_grad_norm  the gradients are scaled down to this norm over all groups (held ones too), and a step with an infinite or NaN gradient changes nothing: decided on the
+                   device, nothing waits.  float("inf"): the check alone.  last_norm() and skipped_last() read the outcome (they wait).
+
+    All groups share one step count; with max_grad_norm it is on the device and counts the steps that were not skipped.  The shN group is held during the first
+    1000 iterations like FusedAdam's (its moments stay zero).  The SH step is not fused into the render backward (begin_fused_sh_step returns None)."""
+
+    def __init__(self, model, lrs, betas=(0.9, 0.999), eps=1e-15, skip_sh_steps=False, weight_decay=None, moments=32, max_grad_norm=None, seed=0):
+        if moments not in (32, 8):
+            raise ValueError("FusedAdamW: moments are kept in 32 or in 8 bits, got %r" % (moments,))
+        unknown = set(weight_decay or {}) - set(GROUPS)
+        if unknown:
+            raise ValueError("FusedAdamW: weight_decay names unknown groups %s; the groups are %s" % (sorted(unknown), ", ".join(GROUPS)))
+        if max_grad_norm is not None and not max_grad_norm > 0:
+            raise ValueError("FusedAdamW: max_grad_norm is positive (inf: the finite check alone), got %r" % (max_grad_norm,))
+        super().__init__(model, lrs, betas, eps, skip_sh_steps)
+        self.weight_decay = {n: float((weight_decay or {}).get(n, 0.0)) for n in GROUPS}
+        self.moments, self.max_grad_norm, self.seed = moments, max_grad_norm, seed
+        self.steps = 0        # calls of step() (with max_grad_norm the block on the device counts those that were not skipped)
+        self.control = None   # ops.step_control, made by the first step
+
+    @staticmethod
+    def for_splat_data(model, means_lr=0.00016, shs_lr=0.0025, scaling_lr=0.005, rotation_lr=0.001, opacity_lr=0.05, scene_scale=1.0, **kw):
+        return FusedAdamW(model, splat_rates(means_lr, shs_lr, scaling_lr, rotation_lr, opacity_lr, scene_scale), **kw)
+
+    # ---- state ---------------------------------------------------------------------------------------------------------
+    def _moments(self, name):
+        """The moments of the tensor that a group belongs to (sh0 and shN share theirs)."""
+        key = _ATTR[name]
+        st = self.state.get(key)
+        if st is None:
+            p = self._param(name)
+            if self.moments == 32:
+                st = {k: torch.zeros(p.shape, dtype=torch.float32, device=p.device) for k in ("exp_avg", "exp_avg_sq")}
+            else:
+                runs = -(-p.numel() // ops.MOMENT_RUN)
+                st = {k: torch.zeros(p.shape, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn) for k in ("exp_avg", "exp_rms")}
+                st.update({k: torch.zeros(runs, dtype=torch.float32, device=p.device) for k in ("avg_scale", "rms_scale")})
+            self.state[key] = st
+        return st
+
+    def moment_values(self, name):
+        """(first, second) moment of the tensor that a group belongs to, as float32 values."""
+        st = self._moments(name)
+        if self.moments == 32:
+            return st["exp_avg"], st["exp_avg_sq"]
+        return decode_moment(st["exp_avg"], st["avg_scale"]), decode_moment(st["exp_rms"], st["rms_scale"]).square()
+
+    def step_count(self, name):
+        return self.steps
+
+    def last_norm(self):
+        return float(self.control[0])
+
+    def skipped_last(self):
+        return bool(self.control[2])
+
+    def reset_state(self, indices):
+        if self.moments == 32:
+            return super().reset_state(indices)
+        for st in self.state.values():   # (a zero code is zero under any scale)
+            for k in ("exp_avg", "exp_rms"):
+                st[k].view(torch.uint8)[indices] = 0
+
+    def extend_state(self, n_new):
+        if self.moments == 32:
+            return super().extend_state(n_new)
+        for st in self.state.values():   # (the runs go on counting through the tensor: the old ones keep their scales, those that begin behind them hold zeros)
+            for k in ("exp_avg", "exp_rms"):
+                z = torch.zeros((n_new,) + tuple(st[k].shape[1:]), dtype=torch.uint8, device=st[k].device)
+                st[k] = torch.cat([st[k].view(torch.uint8), z], 0).view(torch.float8_e4m3fn)
+            for k in ("avg_scale", "rms_scale"):
+                more = -(-st["exp_avg"].numel() // ops.MOMENT_RUN) - st[k].numel()
+                st[k] = torch.cat([st[k], torch.zeros(more, dtype=torch.float32, device=st[k].device)])
+
+    def select_state(self, indices):
+        if self.moments == 32:
+            return super().select_state(indices)
+        self.reindex_generation += 1
+        sts = list(self.state.values())
+        if sts:
+            names = ("exp_avg", "exp_rms", "avg_scale", "rms_scale")
+            new = ops.adamw8_select_rows(*[[st[k] for st in sts] for k in names], indices.contiguous())
+            for k, column in zip(names, new):
+                for st, t in zip(sts, column):
+                    st[k] = t
+
+    # ---- step ------------------------------------------------------------------------------------------------------------
+    def begin_fused_sh_step(self, iteration):
+        return None
+
+    @torch.no_grad()
+    def step(self, iteration, rows=None, skip_sh=False):
+        """One AdamW step of every group that has a gradient; rows as in FusedAdam.step (32-bit moments, no max_grad_norm: a rank sees only its rows' gradients, and
+        runs of 128 do not end where its rows do)."""
+        if skip_sh:
+            raise RuntimeError("FusedAdamW.step(skip_sh=True): the SH step is not fused into the render backward")
+        if rows is not None and (self.moments == 8 or self.max_grad_norm is not None):
+            raise RuntimeError("FusedAdamW.step(rows=...): row sharding needs moments in 32 bits and no max_grad_norm")
+        r = (lambda t: t) if rows is None else (lambda t: t[rows[0]:rows[1]])
+        lr, wd = {g["name"]: g["lr"] for g in self.groups}, self.weight_decay
+        hold = iteration <= 1000 or (self.skip_sh_steps and iteration % 2 != 0 and iteration <= 25000)
+        names = [n for n in GROUPS if n != "shN" and self._param(n).grad is not None]
+        if not names:
+            return
+        self.steps += 1
+        params = [self._param(n) for n in names]
+        grads = [r(p.grad) for p in params]
+        sts = [self._moments(n) for n in names]
+        splits = [(3, lr["shN"], wd["shN"], False, hold) if n == "sh0" and p.shape[1] > 1 else (0, 0.0, 0.0, False, False) for n, p in zip(names, params)]
+        steps = [self.steps] * len(names)
+        if self.max_grad_norm is not None:
+            if self.control is None:
+                self.control = ops.step_control(params[0].device)
+            ops.grad_norm_multi(grads, self.control, self.max_grad_norm)
+            steps = []
+        args = ([lr[n] for n in names], [wd[n] for n in names], self.betas[0], self.betas[1], self.eps, steps)
+        col = lambda k: [r(st[k]) for st in sts]  # noqa: E731
+        control = self.control if not steps else None
+        if self.moments == 32:
+            ops.adamw_step_multi([r(p.data) for p in params], col("exp_avg"), col("exp_avg_sq"), grads, *args, control=control, splits=splits)
+        else:
+            whole = lambda k: [st[k] for st in sts]  # noqa: E731
+            ops.adamw8_step_multi([p.data for p in params], whole("exp_avg"), whole("exp_rms"), whole("avg_scale"), whole("rms_scale"), grads, *args,
+                                  control=control, splits=splits, seed=self.seed)
 
 
 class ExponentialLR:

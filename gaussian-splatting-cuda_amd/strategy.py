@@ -23,7 +23,9 @@ class MCMC:
     NOISE_LR = 5e5   # mcmc.hpp:79
     N_MAX = 51       # binomial table (mcmc.cpp:459-473)
 
-    def __init__(self, model, params: OptimizationParameters, scene_scale: float = 1.0, generator=None):
+    def __init__(self, model, params: OptimizationParameters, scene_scale: float = 1.0, generator=None, make_optimizer=optim.FusedAdam.for_splat_data):
+        """make_optimizer(model, means_lr, shs_lr, scaling_lr, rotation_lr, opacity_lr, scene_scale): the optimizer of the six groups (optim.FusedAdamW.for_splat_data, or
+        a functools.partial of it with its options, for AdamW)."""
         self.model, self.params, self.generator = model, params, generator
         dev = model.means.device
         import numpy as np
@@ -35,8 +37,7 @@ class MCMC:
                     b = np.float32(b * (np.float32(n - i) / np.float32(i + 1)))
                 binoms[n, k] = b
         self.binoms = torch.from_numpy(binoms).to(dev).contiguous()
-        self.optimizer = optim.FusedAdam.for_splat_data(model, params.means_lr, params.shs_lr, params.scaling_lr, params.rotation_lr,
-                                                        params.opacity_lr, scene_scale)
+        self.optimizer = make_optimizer(model, params.means_lr, params.shs_lr, params.scaling_lr, params.rotation_lr, params.opacity_lr, scene_scale)
         self.scheduler = optim.ExponentialLR(self.optimizer, 0.01 ** (1.0 / params.iterations), 0)
         self.on_resize = None   # callback(model) after add_new_gs replaced the parameter tensors (e.g. rebuild the gradient bucket)
         self.before_reindex = None    # callback() before rows are permuted / removed (distributed.ShardedAdam.merge_moments: every rank needs complete moments first)

@@ -10,6 +10,7 @@
 
 One process per GPU; rank r renders camera `cams[(it * world + r) % len(cams)]`.  Every rank holds a full replica and applies
 the identical update (the strategy's random draws come from a generator seeded identically on all ranks)."""
+import functools
 import gc
 import os
 import sys
@@ -19,13 +20,15 @@ import torch.distributed as dist
 
 from . import distributed as gdist
 from . import loss as gloss
+from . import optim
 from . import rasterizer
 from .strategy import MCMC, OptimizationParameters
 
 
 class Trainer:
     def __init__(self, model, cameras, images, params: OptimizationParameters = None, background=None, scene_scale=1.0, seed=0,
-                 sharded_adam=False, exchange="colors", fused_sh_adam=True, guarded_lists=True, fused_regularisers=True):
+                 sharded_adam=False, exchange="colors", fused_sh_adam=True, guarded_lists=True, fused_regularisers=True,
+                 optimizer="adam", optimizer_options=None):
         """cameras: list of rasterizer.Camera; images: list of [3,H,W] ground-truth tensors on the device.
         sharded_adam (world > 1): reduce-scatter -> Adam on this rank's 1/world of the Gaussians -> all-gather of the parameters
         (distributed.ShardedAdam) instead of all-reduce + replicated Adam.
@@ -37,7 +40,16 @@ class Trainer:
         guarded_lists: render with rasterize_fused(guarded=True) — no host read of n_isects per iteration (include/gsx.h "guarded lists");
         an iteration whose intersection lists outgrew their capacity is repeated before its optimizer step (`capacity_misses` counts them).
         fused_regularisers: the gradients of the strategy's scale / opacity regularisers are added inside the render backward's
-        activation-Jacobian kernel (same values as the separate elementwise ops of _add_regularisers up to the rounding of one fma)."""
+        activation-Jacobian kernel (same values as the separate elementwise ops of _add_regularisers up to the rounding of one fma).
+        optimizer: "adam" (optim.FusedAdam), "adamw" or "adamw8" (optim.FusedAdamW with moments in 32 or 8 bits); optimizer_options: FusedAdamW's
+        weight_decay, max_grad_norm, seed, ...  AdamW steps the SH tensor itself (no fused_sh_adam); sharded_adam takes "adamw" without max_grad_norm."""
+        if optimizer not in ("adam", "adamw", "adamw8"):
+            raise ValueError("Trainer: optimizer is 'adam', 'adamw' or 'adamw8', got %r" % (optimizer,))
+        options = dict(optimizer_options or {})
+        if optimizer == "adam" and options:
+            raise ValueError("Trainer: optimizer_options are those of 'adamw' and 'adamw8'")
+        if sharded_adam and (optimizer == "adamw8" or options.get("max_grad_norm") is not None):
+            raise ValueError("Trainer: sharded_adam needs moments in 32 bits and no max_grad_norm")
         self.model, self.cameras = model, cameras
         # dense [3,H,W] once, here: a target that is a permuted view (e.g. a clamped render: torch.clamp keeps the HWC strides of its input) would
         # otherwise be copied by the loss in EVERY iteration (13 MB per frame at 1296x840: 14 us of the garden stand-in's 2.2 ms)
@@ -54,7 +66,8 @@ class Trainer:
             p.requires_grad_(True)
         self.exchange = exchange if (self.multi and not sharded_adam) else None
         self.fused_sh_adam = fused_sh_adam and not sharded_adam and (not self.multi or self.exchange == "colors")
-        self.strategy = MCMC(model, self.params, scene_scale, gen)
+        make = optim.FusedAdam.for_splat_data if optimizer == "adam" else functools.partial(optim.FusedAdamW.for_splat_data, moments=8 if optimizer == "adamw8" else 32, **options)
+        self.strategy = MCMC(model, self.params, scene_scale, gen, make)
         self.strategy.on_resize = self._rebuild_bucket
         self._rebuild_bucket(model)
         self.sharded = gdist.ShardedAdam(self.strategy.optimizer) if (sharded_adam and self.multi) else None

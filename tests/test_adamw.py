@@ -684,3 +684,168 @@ def test_tensors_past_32_bit_offsets(bits):
     at = torch.cat([torch.arange(int(i) * 21, int(i) * 21 + 21) for i in idx.cpu()])
     old = m.view(torch.uint8)[at.cuda()].view(torch.float8_e4m3fn).cpu().double() * sm[at.cuda() // 128].cpu().double()
     ref.check_codes(a[0].cpu().reshape(-1), sa[0].cpu(), old, 2 * ref.U * old.abs(), False, None)
+
+
+# ---- the optimizer of a model --------------------------------------------------------------------------------------------------------------------------------------
+def splat_model(n, K, dev, seed=0):
+    import gsx  # noqa: F401
+    from gsx import rasterizer
+    g = torch.Generator().manual_seed(seed)
+    m = rasterizer.SplatData(means=torch.randn(n, 3, generator=g).to(dev), sh=torch.randn(n, K, 3, generator=g).to(dev), scaling_raw=torch.randn(n, 3, generator=g).to(dev),
+                             rotation_raw=torch.randn(n, 4, generator=g).to(dev), opacity_raw=torch.randn(n, 1, generator=g).to(dev), active_sh_degree=0)
+    for p in m.params():
+        p.requires_grad_(True)
+    return m
+
+
+def test_fused_adamw_refuses_and_keeps_its_books_without_a_gpu():
+    import gsx  # noqa: F401
+    from gsx import optim, parameters, rasterizer, trainer
+    m = splat_model(50, 16, "cpu")
+    mk = lambda **kw: optim.FusedAdamW.for_splat_data(m, **kw)  # noqa: E731
+    for bad in (dict(moments=16), dict(weight_decay={"colour": 0.1}), dict(max_grad_norm=0.0), dict(max_grad_norm=float("nan"))):
+        with pytest.raises(ValueError):
+            mk(**bad)
+    assert [g["lr"] for g in mk().groups] == [g["lr"] for g in optim.FusedAdam.for_splat_data(m).groups]
+    opt = mk(moments=8)
+    assert opt.begin_fused_sh_step(5) is None
+    opt.step(1)                                                     # no gradients: nothing to do
+    assert opt.steps == 0
+    with pytest.raises(RuntimeError, match="skip_sh"):
+        opt.step(1, skip_sh=True)
+    for o in (opt, mk(max_grad_norm=1.0)):
+        with pytest.raises(RuntimeError, match="row sharding"):
+            o.step(1, rows=(0, 10))
+    for name in ("means", "sh0", "opacity"):
+        opt._moments(name)
+    st = opt.state["sh"]
+    assert st["exp_avg"].shape == (50, 16, 3) and st["exp_rms"].dtype == torch.float8_e4m3fn and st["avg_scale"].numel() == -(-50 * 48 // 128)
+    st["exp_avg"].view(torch.uint8).fill_(0x38)                     # ones
+    st["avg_scale"].fill_(2.0)
+    opt.reset_state(torch.tensor([3, 7]))
+    v = opt.moment_values("shN")[0]
+    assert bool((v[[3, 7]] == 0).all()) and bool((v[4:7] == 2).all())
+    opt.extend_state(13)
+    v = opt.moment_values("sh0")[0]
+    assert v.shape == (63, 16, 3) and bool((v[50:] == 0).all()) and bool((v[10:50] == 2).all()) and st["avg_scale"].numel() == -(-63 * 48 // 128)
+    assert opt.state["opacity_raw"]["rms_scale"].numel() == 1 and opt.state["means"]["exp_avg"].shape == (63, 3)
+    cam = rasterizer.Camera(viewmat=torch.eye(4), K=torch.eye(3), width=16, height=16)
+    tr = lambda **kw: trainer.Trainer(m, [cam], [torch.zeros(3, 16, 16)], parameters.OptimizationParameters(), **kw)  # noqa: E731
+    for bad in (dict(optimizer="sgd"), dict(optimizer_options={"seed": 3}), dict(optimizer="adamw8", sharded_adam=True),
+                dict(optimizer="adamw", optimizer_options={"max_grad_norm": 1.0}, sharded_adam=True)):
+        with pytest.raises(ValueError, match="Trainer"):
+            tr(**bad)
+    assert isinstance(tr(optimizer="adamw8", optimizer_options={"seed": 3}).strategy.optimizer, optim.FusedAdamW)
+    assert tr(optimizer="adamw").strategy.optimizer.moments == 32 and type(tr().strategy.optimizer) is optim.FusedAdam
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [1, 9, 16])
+@pytest.mark.parametrize("clip", [None, 0.5, float("inf")])
+def test_fused_adamw_follows_the_plain_form_over_steps(K, clip):
+    """Five steps of a model with 32-bit moments, shN held for the first of them, against the plain form in 64 bits: the parameters' bounds of the steps add up."""
+    import gsx  # noqa: F401
+    from gsx import optim
+    m = splat_model(333, K, "cuda")
+    decay = {"shN": 0.3, "opacity": 0.1}
+    opt = optim.FusedAdamW.for_splat_data(m, weight_decay=decay, max_grad_norm=clip)
+    lr = {g["name"]: g["lr"] for g in opt.groups}
+    names = [("means", "means"), ("sh", "sh0"), ("scaling_raw", "scaling"), ("rotation_raw", "rotation"), ("opacity_raw", "opacity")]
+    want = {a: [getattr(m, a).detach().cpu().double(), 0.0, 0.0, 0.0] for a, _ in names}
+    for t, it in enumerate((1000, 1001, 1002, 1003, 1004), start=1):
+        g = {a: torch.randn(getattr(m, a).shape, generator=torch.Generator().manual_seed(100 * t + i)) * 10.0 ** (i - 2) for i, (a, _) in enumerate(names)}
+        for a, _ in names:
+            getattr(m, a).grad = g[a].cuda()
+        norm = math.sqrt(sum(float((x.double() ** 2).sum()) for x in g.values()))
+        factor = 1.0 if clip is None else float(torch.tensor(min(1.0, clip / (norm + 1e-6)), dtype=torch.float32))
+        opt.step(it)
+        if clip is not None:
+            assert abs(opt.last_norm() - norm) < 1e-10 * norm and not opt.skipped_last()
+        for a, n in names:
+            p, mm, vv, tol = want[a]
+            rate, wd = torch.full(p.shape, lr[n], dtype=torch.float64), torch.full(p.shape, decay.get(n, 0.0), dtype=torch.float64)
+            zero = torch.zeros_like(p)
+            mm, vv, tol = (zero.clone() if isinstance(x, float) else x for x in (mm, vv, tol))
+            live = torch.ones(p.shape, dtype=torch.bool)
+            if a == "sh" and K > 1:
+                rate[:, 1:], wd[:, 1:] = lr["shN"], 0.3
+                live[:, 1:] = it > 1000
+            q, m1, v1, _, pp, _ = ref.adamw(p, g[a].double(), mm, vv, rate, wd, t, factor=factor)
+            # the moments that a step starts from carry up to 8 roundings each for every step before it: t times the bound of one step covers them
+            want[a] = [torch.where(live, q, p), torch.where(live, m1, mm), torch.where(live, v1, vv), torch.where(live, tol + t * pp, tol)]
+    for a, _ in names:
+        err = (getattr(m, a).detach().cpu().double() - want[a][0]).abs()
+        assert bool((err <= want[a][3] + 1e-40).all()), (a, float((err - want[a][3]).max()))
+    assert opt.step_count("means") == 5 and (clip is None or float(opt.control[3]) == 5)
+
+
+@pytest.mark.gpu
+def test_fused_adamw8_through_growth_reordering_pruning_and_relocation():
+    """The 8-bit moments of a model follow its rows: the values move with them, up to one rounding to nearest for every regrouping."""
+    import gsx  # noqa: F401
+    from gsx import optim
+    n = 777
+    m = splat_model(n, 16, "cuda")
+    opt = optim.FusedAdamW.for_splat_data(m, moments=8, max_grad_norm=1.0, seed=3)
+    for t in range(3):
+        for i, p in enumerate(m.params()):
+            p.grad = torch.randn(p.shape, generator=torch.Generator().manual_seed(10 * t + i)).cuda()
+        opt.step(2000 + t)
+    before = {k: [x.cpu() for x in opt.moment_values(k)] for k in ("means", "sh0", "opacity")}
+    dead = torch.tensor([5, 17, 700], device="cuda")
+    opt.reset_state(dead)
+    opt.extend_state(39)
+    order = torch.randperm(n + 39, generator=torch.Generator().manual_seed(4))
+    opt.select_state(order.cuda())
+    assert opt.reindex_generation == 1
+    for k, (a0, v0) in before.items():
+        a, v = (x.cpu() for x in opt.moment_values(k))
+        for old, new, root in ((a0, a, False), (v0.sqrt(), v.sqrt(), True)):
+            full = torch.zeros((n + 39,) + old.shape[1:])
+            full[:n] = old
+            full[dead.cpu()] = 0
+            full = full[order]
+            # a code is off by 2^-4 of the value, or half of the smallest step (2^-10, roots up to 2^-9) of the largest of its run / 448
+            top = torch.nn.functional.pad(full.abs().flatten(), (0, -full.numel() % 128)).view(-1, 128).amax(1).repeat_interleave(128)[:full.numel()].view(full.shape)
+            assert bool(((new - full).abs() <= (2.0 ** -4 + 1e-6) * full.abs() + 2.0 ** -9 / 448 * top * (1 + 1e-6)).all())
+            assert bool((new[full == 0] == 0).all()) and (not root or bool((new[full > 0] > 0).all()))
+    p0 = m.means.detach().clone()
+    m2 = splat_model(n + 39, 16, "cuda", seed=9)
+    opt.model = m2
+    for p in m2.params():
+        p.grad = torch.zeros_like(p)
+    opt.step(2010)
+    assert all(bool(torch.isfinite(p).all()) for p in m2.params()) and p0.shape[0] == n
+    # a NaN gradient: skipped, on the device
+    m2.means.grad[3, 1] = float("nan")
+    kept = [p.detach().clone() for p in m2.params()]
+    codes = opt.state["sh"]["exp_avg"].view(torch.uint8).clone()
+    opt.step(2011)
+    assert opt.skipped_last() and float(opt.control[3]) == 4 and all(torch.equal(a, b) for a, b in zip(kept, m2.params())) and torch.equal(codes, opt.state["sh"]["exp_avg"].view(torch.uint8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("optimizer,options", [("adamw", None), ("adamw", {"max_grad_norm": 0.05, "weight_decay": {"shN": 0.01}}), ("adamw8", {"max_grad_norm": 0.05}), ("adamw8", {"seed": None})])
+def test_training_steps_with_adamw(optimizer, options):
+    """Training through the trainer, with growth, relocation and reordering on the way: finite parameters, moments of the model's size, and the same run twice gives
+    the same moments' sizes and steps."""
+    from tests.test_gpu_training import _scene
+    import gsx  # noqa: F401
+    from gsx import rasterizer, strategy, trainer
+    sc, model, cams = _scene("cuda:0")
+    bg = sc["background"].to("cuda:0")
+    with torch.no_grad():
+        images = [rasterizer.rasterize_fused(c, model, bg).image.clone() for c in cams]
+    model.means = (model.means + 0.01 * torch.randn(model.means.shape, generator=torch.Generator().manual_seed(1)).cuda()).contiguous()
+    n0 = model.means.shape[0]
+    params = strategy.OptimizationParameters(iterations=60, start_refine=10, refine_every=20, stop_refine=50, max_cap=3200)
+    tr = trainer.Trainer(model, cams, images, params, bg, seed=1, optimizer=optimizer, optimizer_options=options)
+    tr.train(60)
+    n = model.means.shape[0]
+    assert n > n0 and all(bool(torch.isfinite(p).all()) for p in model.params())
+    opt = tr.strategy.optimizer
+    for name in ("means", "sh0", "scaling", "rotation", "opacity"):
+        a, v = opt.moment_values(name)
+        assert a.shape[0] == n and bool(torch.isfinite(a).all()) and bool((v >= 0).all()) and float(a.abs().max()) > 0
+    if options and "max_grad_norm" in options:
+        assert float(opt.control[3]) == opt.steps and opt.last_norm() > 0
