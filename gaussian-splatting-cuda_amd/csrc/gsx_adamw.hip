@@ -9,7 +9,7 @@ constexpr uint32_t kChunk = 1024;   // values of one pass of a workgroup: four o
 // the 2 048 workgroups in flight over 150 MB of every array, 5.2.
 constexpr uint32_t kPer = 1;
 
-template <uint32_t L> struct List { Chunks<Rec, L> c; Betas b; };
+template <uint32_t L> struct List { static constexpr uint32_t kRoom = L; Chunks<Rec, L> c; Betas b; };
 
 template <class P, class G, uint32_t L>
 __global__ __launch_bounds__(256) void adamw_kernel(List<L> list) {
@@ -79,13 +79,30 @@ constexpr uint64_t kCacheBytes = 256ull << 20;
 struct NormRec { const void* grad; uint64_t n, cols, ld; };
 struct NormEnd { double* partial; double* control; double max_norm; uint32_t blocks; };   // partial: one for each workgroup of the whole call
 template <uint32_t L> struct NormList {
+    static constexpr uint32_t kRoom = L;
     Chunks<NormRec, L> c;
     NormEnd e;
     uint32_t first;   // this launch's first partial
 };
 
+template <int C> GSX_DEV double dpp_add(double x) {
+    const uint64_t b = (uint64_t)__double_as_longlong(x);
+    const uint32_t low = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, C, 0xF, 0xF, true);
+    const uint32_t high = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), C, 0xF, 0xF, true);
+    return x + __longlong_as_double((long long)((uint64_t)high << 32 | low));
+}
+GSX_DEV double of_lane(double x, int lane) {
+    const uint64_t b = (uint64_t)__double_as_longlong(x);
+    const uint32_t low = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane), high = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+    return __longlong_as_double((long long)((uint64_t)high << 32 | low));
+}
+// Sum over the workgroup, in all of it: within the rows of 16 lanes, over a wave's four rows, over the four waves.
 GSX_DEV double block_sum(double x, double* lds) {
-    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+    x = dpp_add<0xB1>(x);    // neighbours
+    x = dpp_add<0x4E>(x);    // pairs of a quad
+    x = dpp_add<0x141>(x);   // halves of eight
+    x = dpp_add<0x140>(x);   // halves of a row
+    x = (of_lane(x, 0) + of_lane(x, 16)) + (of_lane(x, 32) + of_lane(x, 48));
     __syncthreads();
     if ((threadIdx.x & 63u) == 0) lds[threadIdx.x >> 6] = x;
     __syncthreads();
@@ -165,24 +182,19 @@ __global__ __launch_bounds__(256) void grad_norm_end_kernel(NormEnd e) {
 
 // Calls f(list, workgroups, dtype) for every launch of a norm over these tensors; what the lists hold besides the tensors is f's.
 template <class F> int norm_lists(uint32_t count, const gsx_grad_tensor* tensors, F f) {
-    NormList<kFew> few;
-    NormList<kMany> many;
     uint32_t mask = 0;
     for (uint32_t i = 0; i < count; ++i) mask |= 1u << tensors[i].dtype;
     for (uint32_t d = 0; d <= GSX_DTYPE_F16; ++d) {
         if (!(mask >> d & 1u)) continue;
-        const int rc = launch_lists<NormRec>(
-            count, kNormChunk, [](uint32_t chunks) { return (chunks + kNormGrid - 1) / kNormGrid; }, few.c, many.c,
+        const int rc = launch_lists<NormList, NormRec>(
+            count, kNormChunk, [](uint32_t chunks) { return (chunks + kNormGrid - 1) / kNormGrid; },
             [&](uint32_t i, NormRec* r, uint64_t* n) {
                 const gsx_grad_tensor& x = tensors[i];
                 *n = x.rows * x.cols;
                 *r = NormRec{x.grad, *n, x.cols, x.rows > 1 ? x.ld : x.cols};
                 return x.dtype == d;
             },
-            [&](auto& c, uint32_t blocks) {
-                if constexpr (sizeof(c.rec) == sizeof(few.c.rec)) return f(few, blocks, d);
-                else return f(many, blocks, d);
-            });
+            [&](auto& a, uint32_t blocks) { return f(a, blocks, d); });
         if (rc != GSX_OK) return rc;
     }
     return GSX_OK;
@@ -260,31 +272,26 @@ extern "C" int gsx_adamw_step_multi(uint32_t count, const gsx_adamw_tensor* tens
                                     void* stream) {
     const int bad = check_adamw(count, tensors, beta1, beta2, eps, false, control);
     if (bad != GSX_OK || count == 0) return bad;
-    List<kFew> few;
-    List<kMany> many;
-    few.b = many.b = betas_of(beta1, beta2, eps, 0, control);
+    const Betas betas = betas_of(beta1, beta2, eps, 0, control);
     Corrections last = {};
     const uint32_t mask = types_of(count, tensors);
     for (uint32_t types = 0; types < 9; ++types) {
         if (!(mask >> types & 1u)) continue;
         const uint32_t pd = types / 3, gd = types % 3;
-        const int rc = launch_lists<Rec>(
-            count, kChunk, [](uint32_t) { return kPer; }, few.c, many.c,
+        const int rc = launch_lists<List, Rec>(
+            count, kChunk, [](uint32_t) { return kPer; },
             [&](uint32_t i, Rec* r, uint64_t* n) {
                 if (tensors[i].param_dtype != pd || tensors[i].grad_dtype != gd) return false;
-                *r = rec_of(tensors[i], i, few.b, &last);
+                *r = rec_of(tensors[i], i, betas, &last);
                 *n = r->n;
                 return true;
             },
-            [&](auto& c, uint32_t blocks) {
+            [&](auto& a, uint32_t blocks) {
+                a.b = betas;
                 by_dtype(pd, [&](auto p) {
                     by_dtype(gd, [&](auto g) {
-                        typedef decltype(p) P;
-                        typedef decltype(g) G;
-                        if constexpr (sizeof(c.rec) == sizeof(few.c.rec))
-                            hipLaunchKernelGGL((adamw_kernel<P, G, kFew>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, few);
-                        else
-                            hipLaunchKernelGGL((adamw_kernel<P, G, kMany>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, many);
+                        constexpr uint32_t L = std::remove_reference_t<decltype(a)>::kRoom;
+                        hipLaunchKernelGGL((adamw_kernel<decltype(p), decltype(g), L>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
                     });
                 });
                 return check_launch("adamw_step_multi");
@@ -314,7 +321,7 @@ extern "C" int gsx_grad_norm_multi(uint32_t count, const gsx_grad_tensor* tensor
         a.e = end; a.first = first;
         by_dtype(d, [&](auto g) {
             typedef decltype(g) G;
-            constexpr uint32_t L = sizeof(a.c.rec) / sizeof(NormRec);
+            constexpr uint32_t L = std::remove_reference_t<decltype(a)>::kRoom;
             if (bytes <= kCacheBytes) hipLaunchKernelGGL((grad_norm_kernel<G, L, true>), dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
             else hipLaunchKernelGGL((grad_norm_kernel<G, L, false>), dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
         });

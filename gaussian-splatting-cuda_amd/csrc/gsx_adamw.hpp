@@ -19,9 +19,9 @@ int check_launch(const char* what);
 
 namespace optim {
 
-// A launch's argument block has room for few tensors (a model's parameter groups) or for many (a network's): the smallest that holds the list is taken.  For
-// 150 tensors one launch of many measured 22 us where five of 32 tensors took 48; the large block costs a launch 2 us on the host.
-constexpr uint32_t kFew = 16, kMany = 256;
+// A launch's argument block has room for few tensors (a model's parameter groups), for some or for many (a network's): the smallest that holds the list is
+// taken.  Room for 256 costs a launch 3 us on the host; five launches of 32 tensors for a list of 150 took 48 us, one of 256 takes 17.
+constexpr uint32_t kFew = 16, kSome = 64, kMany = 256;
 
 // Vectors of four values at any address that the type itself may have: gfx950 loads and stores them with one instruction wherever they lie.
 template <class T> struct Vec4;
@@ -79,38 +79,38 @@ inline bool count_of(uint64_t rows, uint64_t cols, uint64_t* n) {
     return true;
 }
 
-// Gathers tensors and launches them: item(i, &rec, &values) is false for a tensor that does not belong to this launch; launch(list) for every full list.  `few` and
-// `many` are the two argument blocks (host); per(chunks): how many of them a workgroup takes.
-template <class R, class Few, class Many, class Per, class Item, class Launch>
-int launch_lists(uint32_t count, uint32_t chunk, Per per, Few& few, Many& many, Item item, Launch launch) {
+// Gathers tensors and launches them: item(i, &rec, &values) is false for a tensor that does not belong here; launch(args, workgroups) for every full list, args an
+// Args<L> (with its tensors in args.c) whose other members are the launch's to fill.  per(chunks): how many of them a workgroup takes.
+template <template <uint32_t> class Args, class R, class Per, class Item, class Launch>
+int launch_lists(uint32_t count, uint32_t chunk, Per per, Item item, Launch launch) {
+    R rec[kMany];
+    uint32_t begin[kMany];
     uint32_t i = 0;
     while (i < count) {
         uint32_t k = 0;
         uint64_t chunks = 0;
         for (; i < count; ++i) {
-            R rec;
             uint64_t n = 0;
-            if (!item(i, &rec, &n) || n == 0) continue;
+            R r;
+            if (!item(i, &r, &n) || n == 0) continue;
             if (k == kMany || (k != 0 && chunks + chunks_of(n, chunk) > kMostChunks)) break;
-            if (k < kFew) {
-                few.rec[k] = rec;
-                few.begin[k] = (uint32_t)chunks;
-            } else {
-                if (k == kFew) { std::copy_n(few.rec, kFew, many.rec); std::copy_n(few.begin, kFew, many.begin); }
-                many.rec[k] = rec;
-                many.begin[k] = (uint32_t)chunks;
-            }
-            ++k;
+            rec[k] = r;
+            begin[k++] = (uint32_t)chunks;
             chunks += chunks_of(n, chunk);
         }
         if (k == 0) break;
-        auto finish = [&](auto& a, uint32_t room) {
-            for (uint32_t j = k; j <= room; ++j) a.begin[j] = 0xFFFFFFFFu;
-            a.chunks = (uint32_t)chunks;
-            a.per = per((uint32_t)chunks);
-            return launch(a, (a.chunks + a.per - 1) / a.per);
+        auto go = [&](auto room) {
+            constexpr uint32_t L = decltype(room)::value;
+            Args<L> a;
+            std::copy_n(rec, k, a.c.rec);
+            std::copy_n(begin, k, a.c.begin);
+            std::fill(a.c.begin + k, a.c.begin + L + 1, 0xFFFFFFFFu);
+            a.c.chunks = (uint32_t)chunks;
+            a.c.per = per(a.c.chunks);
+            return launch(a, (a.c.chunks + a.c.per - 1) / a.c.per);
         };
-        const int rc = k <= kFew ? finish(few, kFew) : finish(many, kMany);
+        const int rc = k <= kFew ? go(std::integral_constant<uint32_t, kFew>{}) : k <= kSome ? go(std::integral_constant<uint32_t, kSome>{})
+                                                                                            : go(std::integral_constant<uint32_t, kMany>{});
         if (rc != GSX_OK) return rc;
     }
     return GSX_OK;

@@ -122,7 +122,7 @@ GSX_DEV void store_codes(uint32_t w, uint8_t* p, uint32_t off, uint32_t count) {
     for (uint32_t j = 0; j < 4 && off + j < count; ++j) p[off + j] = (uint8_t)(w >> (8 * j));
 }
 
-template <uint32_t L> struct List { Chunks<Rec, L> c; Betas b; };
+template <uint32_t L> struct List { static constexpr uint32_t kRoom = L; Chunks<Rec, L> c; Betas b; };
 
 template <class P, class G, bool STOCHASTIC, uint32_t L>
 __global__ __launch_bounds__(256) void adamw8_kernel(List<L> list) {
@@ -214,6 +214,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(List<L> list) {
 // ---- rows of 8-bit moments --------------------------------------------------------------------------------------------------------------------------------
 struct SelectRec { const uint8_t *m, *v; const float *ms, *vs; uint8_t *mo, *vo; float *mso, *vso; uint64_t cols; };
 template <uint32_t L> struct SelectList {
+    static constexpr uint32_t kRoom = L;
     Chunks<SelectRec, L> c;
     const int64_t* index;
     uint64_t rows_in, rows_out;
@@ -347,35 +348,29 @@ extern "C" int gsx_adamw8_step_multi(uint32_t count, const gsx_adamw_tensor* ten
                                      const double* control, void* stream) {
     const int bad = check_adamw(count, tensors, beta1, beta2, eps, true, control);
     if (bad != GSX_OK || count == 0) return bad;
-    List<kFew> few;
-    List<kMany> many;
-    few.b = many.b = betas_of(beta1, beta2, eps, seed, control);
+    const Betas betas = betas_of(beta1, beta2, eps, seed, control);
     Corrections last = {};
     const uint32_t mask = types_of(count, tensors);
     for (uint32_t types = 0; types < 9; ++types) {
         if (!(mask >> types & 1u)) continue;
         const uint32_t pd = types / 3, gd = types % 3;
-        const int rc = launch_lists<Rec>(
-            count, kChunk, per_of, few.c, many.c,
+        const int rc = launch_lists<List, Rec>(
+            count, kChunk, per_of,
             [&](uint32_t i, Rec* r, uint64_t* n) {
                 if (tensors[i].param_dtype != pd || tensors[i].grad_dtype != gd) return false;
-                *r = rec_of(tensors[i], i, few.b, &last);
+                *r = rec_of(tensors[i], i, betas, &last);
                 *n = r->n;
                 return true;
             },
-            [&](auto& c, uint32_t blocks) {
-                auto launch = [&](auto& a, auto p, auto g, auto rounding) {
-                    constexpr uint32_t L = sizeof(a.c.rec) / sizeof(Rec);
-                    hipLaunchKernelGGL((adamw8_kernel<decltype(p), decltype(g), decltype(rounding)::value, L>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
-                };
+            [&](auto& a, uint32_t blocks) {
+                a.b = betas;
+                constexpr uint32_t L = std::remove_reference_t<decltype(a)>::kRoom;
                 by_dtype(pd, [&](auto p) {
                     by_dtype(gd, [&](auto g) {
-                        auto list = [&](auto& a) {
-                            if (stochastic) launch(a, p, g, std::true_type{});
-                            else launch(a, p, g, std::false_type{});
-                        };
-                        if constexpr (sizeof(c.rec) == sizeof(few.c.rec)) list(few);
-                        else list(many);
+                        typedef decltype(p) P;
+                        typedef decltype(g) G;
+                        if (stochastic) hipLaunchKernelGGL((adamw8_kernel<P, G, true, L>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
+                        else hipLaunchKernelGGL((adamw8_kernel<P, G, false, L>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
                     });
                 });
                 return check_launch("adamw8_step_multi");
@@ -396,13 +391,8 @@ extern "C" int gsx_adamw8_select_rows(uint32_t count, const gsx_moments8* tensor
         if (!x.avg_out || !x.rms_out || !x.avg_scale_out || !x.rms_scale_out) return invalid("adamw8_select_rows: null tensor");
         if (rows_in != 0 && (!x.avg_in || !x.rms_in || !x.avg_scale_in || !x.rms_scale_in)) return invalid("adamw8_select_rows: null tensor");
     }
-    SelectList<kFew> few;
-    SelectList<kMany> many;
-    few.index = many.index = index;
-    few.rows_in = many.rows_in = rows_in;
-    few.rows_out = many.rows_out = rows_out;
-    return launch_lists<SelectRec>(
-        count, kSelect, [](uint32_t) { return 1u; }, few.c, many.c,
+    return launch_lists<SelectList, SelectRec>(
+        count, kSelect, [](uint32_t) { return 1u; },
         [&](uint32_t i, SelectRec* r, uint64_t* n) {
             const gsx_moments8& x = tensors[i];
             *r = SelectRec{(const uint8_t*)x.avg_in, (const uint8_t*)x.rms_in, x.avg_scale_in, x.rms_scale_in, (uint8_t*)x.avg_out, (uint8_t*)x.rms_out,
@@ -410,9 +400,10 @@ extern "C" int gsx_adamw8_select_rows(uint32_t count, const gsx_moments8* tensor
             *n = rows_out * x.cols;
             return true;
         },
-        [&](auto& c, uint32_t blocks) {
-            if constexpr (sizeof(c.rec) == sizeof(few.c.rec)) hipLaunchKernelGGL(select_rows_kernel<kFew>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, few);
-            else hipLaunchKernelGGL(select_rows_kernel<kMany>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, many);
+        [&](auto& a, uint32_t blocks) {
+            a.index = index; a.rows_in = rows_in; a.rows_out = rows_out;
+            constexpr uint32_t L = std::remove_reference_t<decltype(a)>::kRoom;
+            hipLaunchKernelGGL(select_rows_kernel<L>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
             return check_launch("adamw8_select_rows");
         });
 }
