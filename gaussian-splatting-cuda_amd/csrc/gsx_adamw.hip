@@ -11,7 +11,7 @@ constexpr uint32_t kPer = 1;
 
 template <uint32_t L> struct List { static constexpr uint32_t kRoom = L; Chunks<Rec, L> c; Betas b; };
 
-template <class P, class G, uint32_t L>
+template <class P, class G, bool HELD, uint32_t L>
 __global__ __launch_bounds__(256) void adamw_kernel(List<L> list) {
     const Betas& a = list.b;
     const Control ctl = control_of(a);
@@ -39,13 +39,15 @@ __global__ __launch_bounds__(256) void adamw_kernel(List<L> list) {
                 }
             }
             uint32_t held = 0;
-            const Steps o = steps_of(k, at.mine, at.cols, whole.value ? nullptr : &held);
+            const Steps o = steps_of(k, at.mine, at.cols, HELD ? &held : nullptr);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float g1 = gv[j] * ctl.factor;
-                mv[j] = a.b1 * mv[j] + a.b1c * g1;
-                vv[j] = a.b2 * vv[j] + a.b2c * g1 * g1;
-                pv[j] = stepped(a, k, o.lrwd[j], o.step[j], pv[j], mv[j], sqrtf(vv[j]));
+                const float g1 = gv[j] * ctl.factor, m1 = a.b1 * mv[j] + a.b1c * g1, v1 = a.b2 * vv[j] + a.b2c * g1 * g1;
+                const float p1 = stepped(a, k, o.lrwd[j], o.step[j], pv[j], m1, sqrtf(v1));
+                const bool keep = HELD && (held >> j & 1u);
+                mv[j] = keep ? mv[j] : m1;
+                vv[j] = keep ? vv[j] : v1;
+                pv[j] = keep ? pv[j] : p1;
             }
             if constexpr (whole.value) {
                 store4(mv, m + off);
@@ -53,7 +55,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(List<L> list) {
                 store4(pv, (P*)r.param + at.base + off);
             } else {
                 for (uint32_t j = 0; j < 4 && off + j < at.count; ++j) {
-                    if (held >> j & 1u) continue;
+                    if (HELD && (held >> j & 1u)) continue;
                     ((P*)r.param)[at(off + j, r.ld_param)] = (P)pv[j];
                     m[off + j] = mv[j];
                     v[off + j] = vv[j];
@@ -275,6 +277,7 @@ extern "C" int gsx_adamw_step_multi(uint32_t count, const gsx_adamw_tensor* tens
     const Betas betas = betas_of(beta1, beta2, eps, 0, control);
     Corrections last = {};
     const uint32_t mask = types_of(count, tensors);
+    const bool held = any_held(count, tensors);
     for (uint32_t types = 0; types < 9; ++types) {
         if (!(mask >> types & 1u)) continue;
         const uint32_t pd = types / 3, gd = types % 3;
@@ -291,7 +294,10 @@ extern "C" int gsx_adamw_step_multi(uint32_t count, const gsx_adamw_tensor* tens
                 by_dtype(pd, [&](auto p) {
                     by_dtype(gd, [&](auto g) {
                         constexpr uint32_t L = std::remove_reference_t<decltype(a)>::kRoom;
-                        hipLaunchKernelGGL((adamw_kernel<decltype(p), decltype(g), L>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
+                        typedef decltype(p) P;
+                        typedef decltype(g) G;
+                        if (held) hipLaunchKernelGGL((adamw_kernel<P, G, true, L>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
+                        else hipLaunchKernelGGL((adamw_kernel<P, G, false, L>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
                     });
                 });
                 return check_launch("adamw_step_multi");

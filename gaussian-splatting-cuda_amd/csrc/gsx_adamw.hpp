@@ -71,6 +71,7 @@ template <class R, uint32_t L, class T> GSX_DEV void walk(const Chunks<R, L>& a,
 inline int invalid(const char* msg) { set_error(msg); return GSX_ERR_INVALID_ARGUMENT; }
 inline uint64_t chunks_of(uint64_t n, uint32_t chunk) { return (n + chunk - 1) / chunk; }
 constexpr uint64_t kMostChunks = 0x7FFFFFFFull;   // of a launch
+constexpr uint32_t kMostBlocks = 1u << 23;        // of a launch: HIP counts its threads in 32 bits
 
 // The number of values of rows x cols, or false where it is beyond what the kernels count.
 inline bool count_of(uint64_t rows, uint64_t cols, uint64_t* n) {
@@ -106,7 +107,7 @@ int launch_lists(uint32_t count, uint32_t chunk, Per per, Item item, Launch laun
             std::copy_n(begin, k, a.c.begin);
             std::fill(a.c.begin + k, a.c.begin + L + 1, 0xFFFFFFFFu);
             a.c.chunks = (uint32_t)chunks;
-            a.c.per = per(a.c.chunks);
+            a.c.per = std::max(per(a.c.chunks), (a.c.chunks + kMostBlocks - 1) / kMostBlocks);
             return launch(a, (a.c.chunks + a.c.per - 1) / a.c.per);
         };
         const int rc = k <= kFew ? go(std::integral_constant<uint32_t, kFew>{}) : k <= kSome ? go(std::integral_constant<uint32_t, kSome>{})
@@ -211,13 +212,13 @@ GSX_DEV float stepped(const Betas& a, const Rates& k, float lrwd, float step, fl
 struct Place {
     const uint64_t n;
     const uint32_t cols;
-    const bool view, by_column, special;
+    const bool view, by_column;
     uint64_t base, row = 0;   // first value of the chunk, and its row (of a view)
     uint32_t col = 0, count;  // its column; values in the chunk
     uint32_t mine = 0;        // column of the lane's first value (of four)
-    bool whole;               // a full chunk, its values one behind the other in all of the tensor's arrays, none of them held
+    bool whole;               // a full chunk, its values one behind the other in all of the tensor's arrays
     GSX_DEV Place(const Rec& r, uint32_t split, uint32_t index, uint32_t chunk)
-        : n(r.n), cols((uint32_t)r.cols), view(r.flags & kRows), by_column(split || view), special(r.flags != 0), base((uint64_t)index * chunk) {
+        : n(r.n), cols((uint32_t)r.cols), view(r.flags & kRows), by_column(split || view), base((uint64_t)index * chunk) {
         if (view || (split && cols > 0xFFFFu)) {
             row = base / r.cols;
             col = (uint32_t)(base - row * r.cols);
@@ -229,7 +230,7 @@ struct Place {
     }
     GSX_DEV void size(uint32_t chunk) {
         count = (uint32_t)std::min<uint64_t>(n - base, chunk);
-        whole = !special && count == chunk;
+        whole = !view && count == chunk;
     }
     GSX_DEV void next(uint32_t chunk) {
         base += chunk;
@@ -249,6 +250,13 @@ struct Place {
         return (row + dr) * ld + (q - dr * cols);
     }
 };
+
+// Whether any of the tensors has a group that is held: kernels of their own (held groups inside the others took 20 registers and two of the six waves).
+inline bool any_held(uint32_t count, const gsx_adamw_tensor* tensors) {
+    for (uint32_t i = 0; i < count; ++i)
+        if (tensors[i].hold || (tensors[i].split && tensors[i].hold_b)) return true;
+    return false;
+}
 
 // The pairs of parameter and gradient types among the tensors: bit 3 * param_dtype + grad_dtype.
 inline uint32_t types_of(uint32_t count, const gsx_adamw_tensor* tensors) {

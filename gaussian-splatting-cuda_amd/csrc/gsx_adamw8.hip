@@ -124,7 +124,7 @@ GSX_DEV void store_codes(uint32_t w, uint8_t* p, uint32_t off, uint32_t count) {
 
 template <uint32_t L> struct List { static constexpr uint32_t kRoom = L; Chunks<Rec, L> c; Betas b; };
 
-template <class P, class G, bool STOCHASTIC, uint32_t L>
+template <class P, class G, bool STOCHASTIC, bool HELD, uint32_t L>
 __global__ __launch_bounds__(256) void adamw8_kernel(List<L> list) {
     const Betas& a = list.b;
     const Control ctl = control_of(a);
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(List<L> list) {
             }
             // (from here on every lane, also those behind the end: the lanes of a run exchange their largest values)
             uint32_t held = 0;
-            const Steps o = steps_of(k, at.mine, at.cols, whole.value ? nullptr : &held);
+            const Steps o = steps_of(k, at.mine, at.cols, HELD ? &held : nullptr);
             f32x4 m1, r1;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -168,8 +168,11 @@ __global__ __launch_bounds__(256) void adamw8_kernel(List<L> list) {
             }
             r1 = roots(r1);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) pv[j] = stepped(a, k, o.lrwd[j], o.step[j], pv[j], m1[j], r1[j]);
-            if constexpr (whole.value) {
+            for (int j = 0; j < 4; ++j) {
+                const float p1 = stepped(a, k, o.lrwd[j], o.step[j], pv[j], m1[j], r1[j]);
+                pv[j] = HELD && (held >> j & 1u) ? pv[j] : p1;
+            }
+            if constexpr (!HELD) {
                 mv = m1;
                 rv = r1;
             } else {
@@ -200,7 +203,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(List<L> list) {
                 store_codes(mw, m, off, at.count);
                 store_codes(vw, v, off, at.count);
                 for (uint32_t j = 0; j < 4 && off + j < at.count; ++j)
-                    if (!(held >> j & 1u)) ((P*)r.param)[at(off + j, r.ld_param)] = (P)pv[j];
+                    if (!HELD || !(held >> j & 1u)) ((P*)r.param)[at(off + j, r.ld_param)] = (P)pv[j];
             }
             if (off < at.count && (off & (GSX_MOMENT_RUN - 1)) == 0) { ms[run] = m_scale; vs[run] = v_scale; }
         };
@@ -351,6 +354,7 @@ extern "C" int gsx_adamw8_step_multi(uint32_t count, const gsx_adamw_tensor* ten
     const Betas betas = betas_of(beta1, beta2, eps, seed, control);
     Corrections last = {};
     const uint32_t mask = types_of(count, tensors);
+    const bool held = any_held(count, tensors);
     for (uint32_t types = 0; types < 9; ++types) {
         if (!(mask >> types & 1u)) continue;
         const uint32_t pd = types / 3, gd = types % 3;
@@ -369,8 +373,11 @@ extern "C" int gsx_adamw8_step_multi(uint32_t count, const gsx_adamw_tensor* ten
                     by_dtype(gd, [&](auto g) {
                         typedef decltype(p) P;
                         typedef decltype(g) G;
-                        if (stochastic) hipLaunchKernelGGL((adamw8_kernel<P, G, true, L>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
-                        else hipLaunchKernelGGL((adamw8_kernel<P, G, false, L>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
+                        auto go = [&](auto rounding, auto holding) {
+                            hipLaunchKernelGGL((adamw8_kernel<P, G, decltype(rounding)::value, decltype(holding)::value, L>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
+                        };
+                        if (stochastic) held ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
+                        else held ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
                     });
                 });
                 return check_launch("adamw8_step_multi");

@@ -15,7 +15,6 @@
 
 #include <ATen/hip/HIPEvent.h>
 
-#include <algorithm>
 #include <atomic>
 #include <chrono>
 #include <cstdlib>
@@ -1232,6 +1231,20 @@ const double* control_of(const at::optional<at::Tensor>& control, const at::Devi
     return control->data_ptr<double>();
 }
 
+// Whether one address is among them twice (none of them null): an open table, four places for each.
+bool repeats(const std::vector<const void*>& addresses) {
+    size_t places = 64;
+    while (places < 4 * addresses.size()) places *= 2;
+    std::vector<const void*> table(places, nullptr);
+    for (const void* a : addresses) {
+        size_t i = (size_t)((uint64_t)(uintptr_t)a * 0x9E3779B97F4A7C15ull >> 20) & (places - 1);
+        while (table[i] != nullptr && table[i] != a) i = (i + 1) & (places - 1);
+        if (table[i] == a) return true;
+        table[i] = a;
+    }
+    return false;
+}
+
 using Splits = std::vector<std::tuple<int64_t, double, double, bool, bool>>;
 
 // What both AdamW operators share; `scales` is empty for moments in 32 bits.
@@ -1253,6 +1266,7 @@ void adamw_multi(const char* op, const TensorList& params, const TensorList& exp
     TORCH_CHECK(!seed.has_value() || (*seed >= 0 && *seed <= 0xFFFFFFFFll), op, ": seed lies in 0 .. 2^32 - 1");
     std::vector<gsx_adamw_tensor> list(k);
     std::vector<const void*> written;
+    written.reserve(3 * k);
     for (size_t i = 0; i < k; ++i) {
         const at::Tensor &p = params[i], &g = grads[i], &m = exp_avgs[i], &v = exp_avg_sqs[i];
         check_on(p, dev, op, "parameter", i); check_on(g, dev, op, "gradient", i); check_on(m, dev, op, "exp_avg", i); check_on(v, dev, op, "exp_avg_sq", i);
@@ -1297,10 +1311,9 @@ void adamw_multi(const char* op, const TensorList& params, const TensorList& exp
             TORCH_CHECK(steps[i] >= 1 && steps[i] <= 0xFFFFFFFFll, op, ": steps count from 1, got ", steps[i], " for parameter ", i);
             x.step = (uint64_t)steps[i];
         }
-        if (p.numel() != 0) written.push_back(x.param);
+        if (p.numel() != 0) written.insert(written.end(), {x.param, x.exp_avg, x.exp_avg_sq});
     }
-    std::sort(written.begin(), written.end());
-    TORCH_CHECK(std::adjacent_find(written.begin(), written.end()) == written.end(), op, ": a parameter is in the list twice");
+    TORCH_CHECK(!repeats(written), op, ": a parameter or a moment is in the lists twice");
     if (eight) check(gsx_adamw8_step_multi((uint32_t)k, list.data(), beta1, beta2, eps, seed.has_value(), (uint32_t)seed.value_or(0), ctl, cur_stream()), op);
     else check(gsx_adamw_step_multi((uint32_t)k, list.data(), beta1, beta2, eps, ctl, cur_stream()), op);
 }

@@ -480,6 +480,25 @@ def test_clipped_steps_follow_the_control_block(bits):
 
 
 @pytest.mark.gpu
+def test_control_block_with_steps_of_the_call_and_without_a_norm():
+    """Explicit steps win over the block's, its factor and skip flag hold all the same; a block that no norm has advanced counts as the first step."""
+    from gsx import ops
+    x = inputs([3000], torch.float32, torch.float32, 14)[0]
+    for c0, steps, step, factor in (([0.0, 0.25, 0.0, 77.0], [5], 5, 0.25), ([0.0, 1.0, 0.0, 0.0], [], 1, 1.0), ([0.0, 0.5, 0.0, 12.0], [], 12, 0.5)):
+        c = ops.step_control("cuda")
+        c[:4] = torch.tensor(c0, dtype=torch.float64)
+        p, m, v = x[0].clone().cuda(), x[2].clone().cuda(), x[3].clone().cuda()
+        ops.adamw_step_multi([p], [m], [v], [x[1].cuda()], [1e-2], [0.1], 0.9, 0.999, 1e-15, steps, control=c)
+        check32(p.cpu(), m.cpu(), v.cpu(), x, 1e-2, 0.1, step, factor=factor)
+    # the device's bias corrections, over the steps where they change most
+    for t in (1, 2, 3, 5, 7, 50, 499, 500, 501, 700, 1000, 5000, 30000):
+        c = ops.step_control("cuda", t)
+        p, m, v = x[0].clone().cuda(), x[2].clone().cuda(), x[3].clone().cuda()
+        ops.adamw_step_multi([p], [m], [v], [x[1].cuda()], [1e-2], [0.0], 0.9, 0.999, 1e-15, [], control=c)
+        check32(p.cpu(), m.cpu(), v.cpu(), x, 1e-2, 0.0, t, what=str(t))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bits", [32, 8])
 def test_captured_steps_replay_like_eager_ones(bits):
     """Norm and update captured on a side stream and replayed, the step advancing on the device, with eager work between the replays."""
@@ -615,6 +634,10 @@ def test_python_entry_points_refuse():
     p = z(4)
     with pytest.raises(RuntimeError, match="twice"):
         ops.adamw_step_multi([p, p], [z(4)] * 2, [z(4)] * 2, [z(4)] * 2, [0.1] * 2, [0.0] * 2, 0.9, 0.999, 1e-8, [1, 1])
+    m = z(4)
+    for two in (dict(exp_avgs=[m, m], exp_avg_sqs=[z(4), z(4)]), dict(exp_avgs=[m, z(4)], exp_avg_sqs=[z(4), m]), dict(exp_avgs=[z(4), z(4)], exp_avg_sqs=[m, m])):
+        with pytest.raises(RuntimeError, match="twice"):
+            ops.adamw_step_multi([z(4), z(4)], two["exp_avgs"], two["exp_avg_sqs"], [z(4)] * 2, [0.1] * 2, [0.0] * 2, 0.9, 0.999, 1e-8, [1, 1])
     with pytest.raises(RuntimeError, match="count from 1"):
         call(z(4), z(4), z(4), z(4), steps=(0,))
     with pytest.raises(RuntimeError, match="control block"):
