@@ -71,11 +71,11 @@ __global__ __launch_bounds__(256) void adamw_kernel(List<L> list) {
 
 // ---- the norm ----------------------------------------------------------------------------------------------------------------------------------------
 constexpr uint32_t kNormVecs = 4, kNormChunk = 1024 * kNormVecs, kNormGrid = 2048;
-// Up to this many workgroups the last one to finish adds the sums up; every one costs 45 ns there (an atomic on one word, and what the release before it
-// waits for: 2 048 of them took 100 of 284 us), a launch of its own 3 us.
-constexpr uint32_t kTickets = 64;
-// Gradients that fit the last-level cache (256 MB) are read to stay there for the update behind the norm: 1 M splats, norm and update 314 us (352 without).  Larger ones
-// stream past it: 295 M values 6.2 TB/s, 5.6 without.
+// Up to this many workgroups the last one to finish adds the sums up; every one costs 45 ns there (an atomic on one word, and what the release before it waits for: 2 048 of
+// them took 100 of 284 us), a launch of its own 3 us.  66 workgroups: 6.0 us in one launch, 7.8 in two; 175: 7.9 and 7.8.
+constexpr uint32_t kTickets = 128;
+// Gradients that fit the last-level cache (256 MB) are read to stay there for the update behind the norm: 1 M splats, norm and update 300 us (330 without; 8-bit moments
+// 195 and 201), the norm alone 47 (43).  Larger ones stream past it: 295 M values 178 us, 203 without.
 constexpr uint64_t kCacheBytes = 256ull << 20;
 
 struct NormRec { const void* grad; uint64_t n, cols, ld; };

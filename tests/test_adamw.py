@@ -872,3 +872,67 @@ def test_training_steps_with_adamw(optimizer, options):
         assert a.shape[0] == n and bool(torch.isfinite(a).all()) and bool((v >= 0).all()) and float(a.abs().max()) > 0
     if options and "max_grad_norm" in options:
         assert float(opt.control[3]) == opt.steps and opt.last_norm() > 0
+
+
+# ---- long lists -----------------------------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [16, 17, 64, 65, 256, 257, 600])
+def test_lists_around_the_argument_blocks_sizes(count):
+    """One tensor more or less than an argument block holds, and several launches; the draws go by the place in the list, wherever the launch begins."""
+    from gsx import ops
+    sizes = [(37 * i) % 301 for i in range(count)]
+    sizes[0], sizes[-1] = 2500, 1029
+    x = inputs(sizes, torch.float32, torch.bfloat16, count)
+    lrs, wds = [1e-3 * (1 + i % 7) for i in range(count)], [0.01 * (i % 3) for i in range(count)]
+    g, c = [t[1].cuda() for t in x], ops.step_control("cuda", 11)
+    ops.grad_norm_multi(g, c)
+    want = math.sqrt(sum(float((t[1].double() ** 2).sum()) for t in x))
+    assert abs(float(c[0]) - want) <= 2.0 ** -36 * want and c[3] == 12 and c[4] == 0
+    p, m, v = [t[0].clone().cuda() for t in x], [t[2].clone().cuda() for t in x], [t[3].clone().cuda() for t in x]
+    ops.adamw_step_multi(p, m, v, g, lrs, wds, 0.9, 0.999, 1e-15, [12] * count)
+    for i in range(count):
+        check32(p[i].cpu(), m[i].cpu(), v[i].cpu(), x[i], lrs[i], wds[i], 12, what=str(i))
+    p = [t[0].clone().cuda() for t in x]
+    mp, rp = [ref.pack(t[2], False) for t in x], [ref.pack(t[4], True) for t in x]
+    m, sm, r, sr = [a.cuda() for a, _ in mp], [b.cuda() for _, b in mp], [a.cuda() for a, _ in rp], [b.cuda() for _, b in rp]
+    ops.adamw8_step_multi(p, m, r, sm, sr, g, lrs, wds, 0.9, 0.999, 1e-15, [], control=c, seed=9)
+    for i in range(count):
+        check8(p[i].cpu(), m[i].cpu(), r[i].cpu(), sm[i].cpu(), sr[i].cpu(), x[i], lrs[i], wds[i], 12, seed=9, ordinal=i, what=str(i))
+    rows = 23
+    y = [inputs([rows * (1 + i % 50)], torch.float32, torch.float32, i)[0] for i in range(count)]
+    mp, rp = [ref.pack(t[2], False) for t in y], [ref.pack(t[4], True) for t in y]
+    index = torch.randperm(rows, generator=torch.Generator().manual_seed(1))[:17]
+    got = ops.adamw8_select_rows([a.cuda().view(rows, -1) for a, _ in mp], [a.cuda().view(rows, -1) for a, _ in rp], [b.cuda() for _, b in mp], [b.cuda() for _, b in rp],
+                                 index.cuda())
+    for i in range(count):
+        old = (mp[i][0].double() * ref.spread(mp[i][1], y[i][2].numel()).double()).view(rows, -1)[index].reshape(-1)
+        ref.check_codes(got[0][i].cpu().reshape(-1), got[2][i].cpu(), old, 2 * ref.U * old.abs(), False, None, str(i))
+
+
+@pytest.mark.gpu
+def test_captured_steps_of_a_long_list():
+    """A captured launch keeps its whole list (30 KB of arguments): replays on the list's buffers equal eager steps."""
+    from gsx import ops
+    x = inputs([100 + i for i in range(100)], torch.float32, torch.float32, 5)
+    k = len(x)
+
+    def fresh():
+        return dict(p=[t[0].clone().cuda() for t in x], g=[t[1].clone().cuda() for t in x], m=[t[2].clone().cuda() for t in x], v=[t[3].clone().cuda() for t in x],
+                    c=ops.step_control("cuda", 4))
+
+    def step(s):
+        ops.grad_norm_multi(s["g"], s["c"], 0.7)
+        ops.adamw_step_multi(s["p"], s["m"], s["v"], s["g"], [1e-2] * k, [0.0] * k, 0.9, 0.999, 1e-15, [], control=s["c"])
+    eager, captured = fresh(), fresh()
+    step(fresh())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(captured)
+    for it in range(4):
+        graph.replay()
+        step(eager)
+        torch.cuda.synchronize()
+        for name in ("p", "m", "v"):
+            assert all(torch.equal(a, b) for a, b in zip(eager[name], captured[name])), (it, name)
+        assert torch.equal(eager["c"], captured["c"])
