@@ -223,7 +223,8 @@ template <uint32_t L> struct SelectList {
     uint64_t rows_in, rows_out;
 };
 
-constexpr uint32_t kSelect = 2048;   // values of one pass of a workgroup (1 M splats 171 us, 181 with 4 096: less LDS, more workgroups at once)
+constexpr uint32_t kSelect = 2048;   // values of a chunk
+constexpr uint32_t kPasses = kSelect / 1024u;
 
 // n / d for n < 2^22, d < 2^22 (the quotient's estimate is off by one at most).
 GSX_DEV uint32_t small_div(uint32_t n, uint32_t d, float rcp) {
@@ -232,68 +233,98 @@ GSX_DEV uint32_t small_div(uint32_t n, uint32_t d, float rcp) {
     return n - q * d >= d ? q + 1u : q;
 }
 
-// A chunk of the new moments is gathered into LDS in pieces of one row (an index, two loads of codes and two scales a piece, whatever the rows' length and the places where
-// old and new runs begin), then coded from there like the update's.  A piece has W = 16 values where the rows' length is a multiple of 16 (the SH coefficients of degree
-// 3: 48), then no piece crosses the end of a run either; else up to four.
-// What bounds it: two dependent loads from random places, of which a row of 48 bytes costs 121 of the memory's (455 MB for 1 M splats, 122 MB of codes).
-template <uint32_t W> struct Codes { uint32_t m[W / 4], v[W / 4]; };
-template <uint32_t W, uint32_t BATCH>
-GSX_DEV void gather(const SelectRec& r, const int64_t* __restrict__ index, uint64_t rows_in, uint64_t row0, uint32_t col0, uint32_t count, float (*lds)[kSelect]) {
-    const uint32_t cols = (uint32_t)r.cols, pieces = (cols + W - 1) / W, last = col0 + count - 1u;
+// Codes four new values of each moment and stores them; off: the first of them in the chunk.  Every lane of the wave takes part, those behind the end with zeros.
+GSX_DEV void store_selected(const SelectRec& r, uint64_t base, uint32_t off, uint32_t count, f32x4 m, f32x4 v) {
+    float m_scale, v_scale;
+    scales_of(m, v, &m_scale, &v_scale);
+    if (off >= count) return;
+    const uint32_t mw = encode4<false, false>(m, m_scale, nullptr), vw = encode4<true, false>(v, v_scale, nullptr);
+    if (off + 4 <= count) {
+        *reinterpret_cast<u32_any*>(r.mo + base + off) = mw;
+        *reinterpret_cast<u32_any*>(r.vo + base + off) = vw;
+    } else {
+        store_codes(mw, r.mo + base, off, count);
+        store_codes(vw, r.vo + base, off, count);
+    }
+    if ((off & (GSX_MOMENT_RUN - 1)) == 0) { r.mso[(base + off) / GSX_MOMENT_RUN] = m_scale; r.vso[(base + off) / GSX_MOMENT_RUN] = v_scale; }
+}
+
+// Rows whose length is a multiple of four: a lane's four values come from one row and one run, straight into its registers.
+GSX_DEV void select_fours(const SelectRec& r, const int64_t* __restrict__ index, uint64_t rows_in, uint64_t base, uint64_t row0, uint32_t col0, uint32_t count) {
+    const uint32_t cols = (uint32_t)r.cols;
+    const bool small = cols < (1u << 21);
+    const float rcp = 1.0f / (float)cols;
+    uint32_t mw[kPasses], vw[kPasses], c[kPasses];
+    float ms[kPasses], vs[kPasses];
+    int64_t src[kPasses];
+#pragma unroll
+    for (uint32_t u = 0; u < kPasses; ++u) {
+        const uint32_t q = col0 + std::min(u * 1024u + threadIdx.x * 4u, count - 4u), dr = small ? small_div(q, cols, rcp) : q / cols;
+        c[u] = q - dr * cols;
+        src[u] = index[row0 + dr];
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < kPasses; ++u) {
+        mw[u] = vw[u] = 0;
+        ms[u] = vs[u] = 0.0f;
+        if (src[u] < 0 || (uint64_t)src[u] >= rows_in || u * 1024u + threadIdx.x * 4u >= count) continue;
+        const uint64_t at = (uint64_t)src[u] * cols + c[u];
+        mw[u] = *reinterpret_cast<const u32_any*>(r.m + at);
+        vw[u] = *reinterpret_cast<const u32_any*>(r.v + at);
+        ms[u] = r.ms[at / GSX_MOMENT_RUN];
+        vs[u] = r.vs[at / GSX_MOMENT_RUN];
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < kPasses; ++u) store_selected(r, base, u * 1024u + threadIdx.x * 4u, count, decode4(mw[u], ms[u]), decode4(vw[u], vs[u]));
+}
+
+// Other rows: a chunk is gathered into LDS in pieces of up to four values of one row (an index, two words of codes and two scales or four a piece, wherever old and new
+// runs begin), and coded from there.
+constexpr uint32_t kBatch = 3;   // pieces of a lane whose loads are in flight together
+GSX_DEV void select_pieces(const SelectRec& r, const int64_t* __restrict__ index, uint64_t rows_in, uint64_t base, uint64_t row0, uint32_t col0, uint32_t count,
+                           float (*lds)[kSelect]) {
+    const uint32_t cols = (uint32_t)r.cols, pieces = (cols + 3) / 4, last = col0 + count - 1u;
     const uint64_t n_in = rows_in * r.cols;
-    const uint32_t items = last / cols * pieces + last % cols / W + 1u;   // pieces from the start of the first row to the last value
+    const uint32_t items = last / cols * pieces + last % cols / 4u + 1u;   // pieces from the start of the first row to the last value
     const bool small = items < (1u << 22) && pieces < (1u << 22);
     const float rcp = 1.0f / (float)pieces;
-    for (uint32_t i = col0 / W + threadIdx.x; i < items; i += 256u * BATCH) {
-        uint32_t c[BATCH], len[BATCH], left[BATCH];
-        int32_t to[BATCH];   // where in the chunk a piece goes; the first may start before it and the last end behind it
-        int64_t src[BATCH];
-        Codes<W> w[BATCH];
-        float m0[BATCH], v0[BATCH], m1[BATCH], v1[BATCH];
+    __syncthreads();
+    for (uint32_t i = col0 / 4u + threadIdx.x; i < items; i += 256u * kBatch) {
+        uint32_t c[kBatch], len[kBatch], left[kBatch], mw[kBatch], vw[kBatch];
+        int32_t to[kBatch];   // where in the chunk a piece goes; the first may start before it and the last end behind it
+        int64_t src[kBatch];
+        float m0[kBatch], v0[kBatch], m1[kBatch], v1[kBatch];
 #pragma unroll
-        for (uint32_t b = 0; b < BATCH; ++b) {
+        for (uint32_t b = 0; b < kBatch; ++b) {
             const uint32_t item = std::min(i + 256u * b, items - 1u), dr = small ? small_div(item, pieces, rcp) : item / pieces;
-            c[b] = (item - dr * pieces) * W;
-            len[b] = std::min(cols - c[b], W);
+            c[b] = (item - dr * pieces) * 4u;
+            len[b] = std::min(cols - c[b], 4u);
             to[b] = (int32_t)(dr * cols + c[b] - col0);
             src[b] = index[row0 + dr];
         }
 #pragma unroll
-        for (uint32_t b = 0; b < BATCH; ++b) {
-            w[b] = Codes<W>{};
+        for (uint32_t b = 0; b < kBatch; ++b) {
+            mw[b] = vw[b] = 0;
             m0[b] = v0[b] = m1[b] = v1[b] = 0.0f;
-            left[b] = W;
+            left[b] = 4;
             if (src[b] < 0 || (uint64_t)src[b] >= rows_in) continue;
             const uint64_t at = (uint64_t)src[b] * cols + c[b], run = at / GSX_MOMENT_RUN;
-            if (W == 16 || at + 4 <= n_in) {
-#pragma unroll
-                for (uint32_t k = 0; k < W / 4; ++k) {
-                    w[b].m[k] = reinterpret_cast<const u32_any*>(r.m + at)[k];
-                    w[b].v[k] = reinterpret_cast<const u32_any*>(r.v + at)[k];
-                }
+            if (at + 4 <= n_in) {
+                mw[b] = *reinterpret_cast<const u32_any*>(r.m + at);
+                vw[b] = *reinterpret_cast<const u32_any*>(r.v + at);
             } else {
-                w[b].m[0] = load_codes(r.m + at, 0, len[b]);
-                w[b].v[0] = load_codes(r.v + at, 0, len[b]);
+                mw[b] = load_codes(r.m + at, 0, len[b]);
+                vw[b] = load_codes(r.v + at, 0, len[b]);
             }
             m0[b] = r.ms[run];
             v0[b] = r.vs[run];
-            if (W == 4) {
-                left[b] = GSX_MOMENT_RUN - (uint32_t)(at % GSX_MOMENT_RUN);   // values up to the next run
-                if (left[b] < len[b]) { m1[b] = r.ms[run + 1]; v1[b] = r.vs[run + 1]; }
-            }
+            left[b] = GSX_MOMENT_RUN - (uint32_t)(at % GSX_MOMENT_RUN);   // values up to the next run
+            if (left[b] < len[b]) { m1[b] = r.ms[run + 1]; v1[b] = r.vs[run + 1]; }
         }
 #pragma unroll
-        for (uint32_t b = 0; b < BATCH; ++b) {
+        for (uint32_t b = 0; b < kBatch; ++b) {
             if (i + 256u * b >= items) continue;
-            if (W == 16) {
-#pragma unroll
-                for (uint32_t k = 0; k < W / 4; ++k) {
-                    *reinterpret_cast<f32x4*>(&lds[0][to[b] + 4 * k]) = decode4(w[b].m[k], m0[b]);
-                    *reinterpret_cast<f32x4*>(&lds[1][to[b] + 4 * k]) = decode4(w[b].v[k], v0[b]);
-                }
-                continue;
-            }
-            const f32x4 mv = decode4(w[b].m[0], 1.0f), rv = decode4(w[b].v[0], 1.0f);
+            const f32x4 mv = decode4(mw[b], 1.0f), rv = decode4(vw[b], 1.0f);
 #pragma unroll
             for (int32_t j = 0; j < 4; ++j) {
                 if (j < (int32_t)len[b] && to[b] + j >= 0 && to[b] + j < (int32_t)count) {
@@ -303,40 +334,30 @@ GSX_DEV void gather(const SelectRec& r, const int64_t* __restrict__ index, uint6
             }
         }
     }
+    __syncthreads();
+    for (uint32_t u = 0; u < kPasses; ++u) {
+        const uint32_t off = u * 1024u + threadIdx.x * 4u;
+        f32x4 m = *reinterpret_cast<const f32x4*>(&lds[0][off]), v = *reinterpret_cast<const f32x4*>(&lds[1][off]);
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            m[j] = off + j < count ? m[j] : 0.0f;
+            v[j] = off + j < count ? v[j] : 0.0f;
+        }
+        store_selected(r, base, off, count, m, v);
+    }
 }
 
-template <uint32_t L> __global__ __launch_bounds__(256) void select_rows_kernel(SelectList<L> a) {
+// What bounds it: rows at random places of memory that comes in lines of 128 bytes.  1 M splats by a random order (122 MB of codes) miss the L2s 8.5 M times, a gigabyte, in
+// 171 us: rows of 48 bytes 85 of them, one to four bytes, of which every L2 fetches every line, the rest.  In an order near the old one, as a growth step's is: 81 us.
+template <uint32_t L> __global__ __launch_bounds__(256, 8) void select_rows_kernel(SelectList<L> a) {
     __shared__ __align__(16) float lds[2][kSelect];
     walk(a.c, [&](const SelectRec& r, uint32_t chunk, uint32_t stop) {
         const uint64_t n = a.rows_out * r.cols;
         for (; chunk < stop; ++chunk) {
             const uint64_t base = (uint64_t)chunk * kSelect, row0 = base >> 32 ? base / r.cols : (uint32_t)base / (uint32_t)r.cols;
             const uint32_t count = (uint32_t)std::min<uint64_t>(n - base, kSelect), col0 = (uint32_t)(base - row0 * r.cols);
-            __syncthreads();
-            if (r.cols % 16 == 0) gather<16, 1>(r, a.index, a.rows_in, row0, col0, count, lds);
-            else gather<4, 3>(r, a.index, a.rows_in, row0, col0, count, lds);
-            __syncthreads();
-            for (uint32_t pass = 0; pass < kSelect; pass += 1024u) {   // (the same number of passes for every lane: the runs' lanes exchange their largest values)
-                const uint32_t off = pass + threadIdx.x * 4u;
-                f32x4 mv = *reinterpret_cast<const f32x4*>(&lds[0][off]), rv = *reinterpret_cast<const f32x4*>(&lds[1][off]);
-#pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    mv[j] = off + j < count ? mv[j] : 0.0f;
-                    rv[j] = off + j < count ? rv[j] : 0.0f;
-                }
-                float m_scale, v_scale;
-                scales_of(mv, rv, &m_scale, &v_scale);
-                if (off >= count) continue;
-                const uint32_t mw = encode4<false, false>(mv, m_scale, nullptr), vw = encode4<true, false>(rv, v_scale, nullptr);
-                if (off + 4 <= count) {
-                    *reinterpret_cast<u32_any*>(r.mo + base + off) = mw;
-                    *reinterpret_cast<u32_any*>(r.vo + base + off) = vw;
-                } else {
-                    store_codes(mw, r.mo + base, off, count);
-                    store_codes(vw, r.vo + base, off, count);
-                }
-                if ((off & (GSX_MOMENT_RUN - 1)) == 0) { r.mso[(base + off) / GSX_MOMENT_RUN] = m_scale; r.vso[(base + off) / GSX_MOMENT_RUN] = v_scale; }
-            }
+            if (r.cols % 4 == 0) select_fours(r, a.index, a.rows_in, base, row0, col0, count);
+            else select_pieces(r, a.index, a.rows_in, base, row0, col0, count, lds);
         }
     });
 }
