@@ -19,52 +19,47 @@ __global__ __launch_bounds__(256) void adamw_kernel(List<L> list) {
     walk(list.c, [&](const Rec& r, uint32_t chunk, uint32_t stop) {
         const Rates k = rates_of(r, ctl);
         Place at(r, k.split, chunk, kChunk);
-        auto pass = [&](auto whole) {   // (compiled twice: the ends of tensors and the views stay out of the way of the whole chunks)
-            const uint32_t off = threadIdx.x * 4u;
+        for (; chunk < stop; ++chunk, at.next(kChunk)) {
             float* m = (float*)r.m + at.base; float* v = (float*)r.v + at.base;
-            f32x4 pv, gv, mv, vv;
-            if constexpr (whole.value) {
-                gv = load4((const G*)r.grad + at.base + off);
-                mv = load4(m + off);
-                vv = load4(v + off);
-                pv = load4((const P*)r.param + at.base + off);
-            } else {   // the end of a tensor, or a view: value by value, all loads at once, none behind the end
+            if (at.whole) {
+                const uint32_t off = threadIdx.x * 4u;
+                f32x4 gv = load4((const G*)r.grad + at.base + off), mv = load4(m + off), vv = load4(v + off), pv = load4((const P*)r.param + at.base + off);
+                uint32_t held = 0;
+                const Steps o = steps_of(k, at.mine, at.cols, HELD ? &held : nullptr);
 #pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    const uint32_t i = std::min(off + j, at.count - 1u);
-                    gv[j] = (float)((const G*)r.grad)[at(i, r.ld_grad)];
-                    pv[j] = (float)((const P*)r.param)[at(i, r.ld_param)];
-                    mv[j] = m[i];
-                    vv[j] = v[i];
+                for (int j = 0; j < 4; ++j) {
+                    const float g1 = gv[j] * ctl.factor, m1 = a.b1 * mv[j] + a.b1c * g1, v1 = a.b2 * vv[j] + a.b2c * g1 * g1;
+                    const float p1 = stepped(a, k, o.lrwd[j], o.step[j], pv[j], m1, sqrtf(v1));
+                    const bool keep = HELD && (held >> j & 1u);
+                    mv[j] = keep ? mv[j] : m1;
+                    vv[j] = keep ? vv[j] : v1;
+                    pv[j] = keep ? pv[j] : p1;
                 }
-            }
-            uint32_t held = 0;
-            const Steps o = steps_of(k, at.mine, at.cols, HELD ? &held : nullptr);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float g1 = gv[j] * ctl.factor, m1 = a.b1 * mv[j] + a.b1c * g1, v1 = a.b2 * vv[j] + a.b2c * g1 * g1;
-                const float p1 = stepped(a, k, o.lrwd[j], o.step[j], pv[j], m1, sqrtf(v1));
-                const bool keep = HELD && (held >> j & 1u);
-                mv[j] = keep ? mv[j] : m1;
-                vv[j] = keep ? vv[j] : v1;
-                pv[j] = keep ? pv[j] : p1;
-            }
-            if constexpr (whole.value) {
                 store4(mv, m + off);
                 store4(vv, v + off);
                 store4(pv, (P*)r.param + at.base + off);
-            } else {
-                for (uint32_t j = 0; j < 4 && off + j < at.count; ++j) {
-                    if (HELD && (held >> j & 1u)) continue;
-                    ((P*)r.param)[at(off + j, r.ld_param)] = (P)pv[j];
-                    m[off + j] = mv[j];
-                    v[off + j] = vv[j];
-                }
+                continue;
             }
-        };
-        for (; chunk < stop; ++chunk, at.next(kChunk)) {
-            if (at.whole) pass(std::true_type{});
-            else pass(std::false_type{});
+            // the end of a tensor, or a view: neighbouring values to neighbouring lanes, all loads of a lane at once, none behind the end
+            float gv[4], mv[4], vv[4], pv[4];
+            Place::Spot s[4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                s[j] = at.spot(std::min(j * 256u + threadIdx.x, at.count - 1u));
+                gv[j] = (float)((const G*)r.grad)[at(s[j], r.ld_grad)];
+                pv[j] = (float)((const P*)r.param)[at(s[j], r.ld_param)];
+                mv[j] = m[s[j].i];
+                vv[j] = v[s[j].i];
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                const bool b = k.split && s[j].c >= k.split;
+                if (j * 256u + threadIdx.x >= at.count || (HELD && (k.flags & (b ? kHoldB : kHold)))) continue;
+                const float g1 = gv[j] * ctl.factor, m1 = a.b1 * mv[j] + a.b1c * g1, v1 = a.b2 * vv[j] + a.b2c * g1 * g1;
+                ((P*)r.param)[at(s[j], r.ld_param)] = (P)stepped(a, k, b ? k.lrwd_b : k.lrwd, b ? k.step_b : k.step, pv[j], m1, sqrtf(v1));
+                m[s[j].i] = m1;
+                v[s[j].i] = v1;
+            }
         }
     });
 }

@@ -243,12 +243,14 @@ struct Place {
         }
         size(chunk);   // (behind the last chunk: not used)
     }
-    // Where value i of the chunk is in an array whose rows are ld apart if the tensor is a view.
-    GSX_DEV uint64_t operator()(uint32_t i, uint64_t ld) const {
-        if (!view) return base + i;
+    // Value i of the chunk: its column, and where it is in an array whose rows are ld apart if the tensor is a view.
+    struct Spot { uint32_t i, dr, c; };
+    GSX_DEV Spot spot(uint32_t i) const {
+        if (!by_column) return {i, 0, 0};
         const uint32_t q = col + i, dr = q / cols;
-        return (row + dr) * ld + (q - dr * cols);
+        return {i, dr, q - dr * cols};
     }
+    GSX_DEV uint64_t operator()(Spot s, uint64_t ld) const { return view ? (row + s.dr) * ld + s.c : base + s.i; }
 };
 
 // Whether any of the tensors has a group that is held: kernels of their own (held groups inside the others took 20 registers and two of the six waves).

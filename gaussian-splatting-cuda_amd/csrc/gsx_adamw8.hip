@@ -148,10 +148,10 @@ __global__ __launch_bounds__(256) void adamw8_kernel(List<L> list) {
                 const uint32_t mw = load_codes(m, off, at.count), vw = load_codes(v, off, at.count), here = std::min(off, at.count - 1u) / GSX_MOMENT_RUN;
 #pragma unroll
                 for (uint32_t j = 0; j < 4; ++j) {
-                    const uint32_t i = std::min(off + j, at.count - 1u);
-                    const float g1 = (float)((const G*)r.grad)[at(i, r.ld_grad)];
+                    const Place::Spot s = at.spot(std::min(off + j, at.count - 1u));
+                    const float g1 = (float)((const G*)r.grad)[at(s, r.ld_grad)];
                     gv[j] = off + j < at.count ? g1 : 0.0f;
-                    pv[j] = (float)((const P*)r.param)[at(i, r.ld_param)];
+                    pv[j] = (float)((const P*)r.param)[at(s, r.ld_param)];
                 }
                 mv = decode4(mw, ms[here]);
                 rv = decode4(vw, vs[here]);
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(List<L> list) {
                 store_codes(mw, m, off, at.count);
                 store_codes(vw, v, off, at.count);
                 for (uint32_t j = 0; j < 4 && off + j < at.count; ++j)
-                    if (!HELD || !(held >> j & 1u)) ((P*)r.param)[at(off + j, r.ld_param)] = (P)pv[j];
+                    if (!HELD || !(held >> j & 1u)) ((P*)r.param)[at(at.spot(off + j), r.ld_param)] = (P)pv[j];
             }
             if (off < at.count && (off & (GSX_MOMENT_RUN - 1)) == 0) { ms[run] = m_scale; vs[run] = v_scale; }
         };
