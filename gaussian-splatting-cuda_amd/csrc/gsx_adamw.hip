@@ -286,16 +286,16 @@ extern "C" int gsx_adamw_step_multi(uint32_t count, const gsx_adamw_tensor* tens
             },
             [&](auto& a, uint32_t blocks) {
                 a.b = betas;
+                int rc = GSX_OK;
                 by_dtype(pd, [&](auto p) {
                     by_dtype(gd, [&](auto g) {
                         constexpr uint32_t L = std::remove_reference_t<decltype(a)>::kRoom;
                         typedef decltype(p) P;
                         typedef decltype(g) G;
-                        if (held) hipLaunchKernelGGL((adamw_kernel<P, G, true, L>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
-                        else hipLaunchKernelGGL((adamw_kernel<P, G, false, L>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
+                        rc = launch_list(held ? adamw_kernel<P, G, true, L> : adamw_kernel<P, G, false, L>, a, blocks, stream, "adamw_step_multi");
                     });
                 });
-                return check_launch("adamw_step_multi");
+                return rc;
             });
         if (rc != GSX_OK) return rc;
     }
@@ -320,14 +320,14 @@ extern "C" int gsx_grad_norm_multi(uint32_t count, const gsx_grad_tensor* tensor
     uint32_t first = 0;
     auto launch = [&](auto& a, uint32_t grid, uint32_t d) {
         a.e = end; a.first = first;
+        int rc = GSX_OK;
         by_dtype(d, [&](auto g) {
             typedef decltype(g) G;
             constexpr uint32_t L = std::remove_reference_t<decltype(a)>::kRoom;
-            if (bytes <= kCacheBytes) hipLaunchKernelGGL((grad_norm_kernel<G, L, true>), dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
-            else hipLaunchKernelGGL((grad_norm_kernel<G, L, false>), dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
+            rc = launch_list(bytes <= kCacheBytes ? grad_norm_kernel<G, L, true> : grad_norm_kernel<G, L, false>, a, grid, stream, "grad_norm_multi");
         });
         first += grid;
-        return check_launch("grad_norm_multi");
+        return rc;
     };
     int rc = norm_lists(count, tensors, launch);
     if (rc == GSX_OK && first == 0) {   // nothing to add up: the norm is zero

@@ -75,9 +75,7 @@ constexpr uint32_t kMostBlocks = 1u << 23;        // of a launch: HIP counts its
 
 // The number of values of rows x cols, or false where it is beyond what the kernels count.
 inline bool count_of(uint64_t rows, uint64_t cols, uint64_t* n) {
-    if (rows != 0 && cols > (1ull << 40) / rows) return false;
-    *n = rows * cols;
-    return true;
+    return !__builtin_mul_overflow(rows, cols, n) && *n <= 1ull << 40;
 }
 
 // Gathers tensors and launches them: item(i, &rec, &values) is false for a tensor that does not belong here; launch(args, workgroups) for every full list, args an
@@ -115,6 +113,13 @@ int launch_lists(uint32_t count, uint32_t chunk, Per per, Item item, Launch laun
         if (rc != GSX_OK) return rc;
     }
     return GSX_OK;
+}
+
+// Launches a kernel whose one argument is a list, from where the list lies (the launch expression would copy its 2 to 32 KB once more).
+template <class A> int launch_list(void (*kernel)(A), A& list, uint32_t blocks, void* stream, const char* what) {
+    void* args[] = {&list};
+    (void)hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3(blocks), dim3(256), args, 0, (hipStream_t)stream);
+    return check_launch(what);
 }
 
 template <class F> void by_dtype(uint32_t d, F f) {

@@ -390,18 +390,17 @@ extern "C" int gsx_adamw8_step_multi(uint32_t count, const gsx_adamw_tensor* ten
             [&](auto& a, uint32_t blocks) {
                 a.b = betas;
                 constexpr uint32_t L = std::remove_reference_t<decltype(a)>::kRoom;
+                int rc = GSX_OK;
                 by_dtype(pd, [&](auto p) {
                     by_dtype(gd, [&](auto g) {
                         typedef decltype(p) P;
                         typedef decltype(g) G;
-                        auto go = [&](auto rounding, auto holding) {
-                            hipLaunchKernelGGL((adamw8_kernel<P, G, decltype(rounding)::value, decltype(holding)::value, L>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
-                        };
-                        if (stochastic) held ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
-                        else held ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
+                        const auto kernel = stochastic ? (held ? adamw8_kernel<P, G, true, true, L> : adamw8_kernel<P, G, true, false, L>)
+                                                       : (held ? adamw8_kernel<P, G, false, true, L> : adamw8_kernel<P, G, false, false, L>);
+                        rc = launch_list(kernel, a, blocks, stream, "adamw8_step_multi");
                     });
                 });
-                return check_launch("adamw8_step_multi");
+                return rc;
             });
         if (rc != GSX_OK) return rc;
     }
@@ -431,7 +430,6 @@ extern "C" int gsx_adamw8_select_rows(uint32_t count, const gsx_moments8* tensor
         [&](auto& a, uint32_t blocks) {
             a.index = index; a.rows_in = rows_in; a.rows_out = rows_out;
             constexpr uint32_t L = std::remove_reference_t<decltype(a)>::kRoom;
-            hipLaunchKernelGGL(select_rows_kernel<L>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
-            return check_launch("adamw8_select_rows");
+            return launch_list(select_rows_kernel<L>, a, blocks, stream, "adamw8_select_rows");
         });
 }

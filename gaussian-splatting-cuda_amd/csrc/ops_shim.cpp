@@ -1195,6 +1195,11 @@ struct TensorList {
     size_t size() const { return t.size(); }
     const at::Tensor& operator[](size_t i) const { return *t[i]; }
 };
+// Lists of numbers and of column groups, read without pybind's casters (three lists of 150: 8 us of a step's 17).
+struct Numbers { std::vector<double> v; };
+struct Counts { std::vector<int64_t> v; };
+struct Split { int64_t split; double lr_b, weight_decay_b; bool hold_a, hold_b; };
+struct Splits { std::vector<Split> v; };
 
 namespace {
 
@@ -1245,16 +1250,15 @@ bool repeats(const std::vector<const void*>& addresses) {
     return false;
 }
 
-using Splits = std::vector<std::tuple<int64_t, double, double, bool, bool>>;
 
 // What both AdamW operators share; `scales` is empty for moments in 32 bits.
 void adamw_multi(const char* op, const TensorList& params, const TensorList& exp_avgs, const TensorList& exp_avg_sqs,
                  const TensorList& avg_scales, const TensorList& rms_scales, bool eight, const TensorList& grads,
-                 const std::vector<double>& lrs, const std::vector<double>& weight_decays, double beta1, double beta2, double eps,
-                 const std::vector<int64_t>& steps, const at::optional<at::Tensor>& control, const Splits& splits, const at::optional<int64_t>& seed) {
+                 const Numbers& lrs, const Numbers& weight_decays, double beta1, double beta2, double eps,
+                 const Counts& steps, const at::optional<at::Tensor>& control, const Splits& splits, const at::optional<int64_t>& seed) {
     const size_t k = params.size();
-    TORCH_CHECK(exp_avgs.size() == k && exp_avg_sqs.size() == k && grads.size() == k && lrs.size() == k && weight_decays.size() == k &&
-                (steps.empty() || steps.size() == k) && (splits.empty() || splits.size() == k) && (!eight || (avg_scales.size() == k && rms_scales.size() == k)),
+    TORCH_CHECK(exp_avgs.size() == k && exp_avg_sqs.size() == k && grads.size() == k && lrs.v.size() == k && weight_decays.v.size() == k &&
+                (steps.v.empty() || steps.v.size() == k) && (splits.v.empty() || splits.v.size() == k) && (!eight || (avg_scales.size() == k && rms_scales.size() == k)),
                 op, ": the lists have one entry for each of the ", k, " parameters (steps and splits may be empty)");
     TORCH_CHECK(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, op, ": betas lie in [0, 1), got ", beta1, ", ", beta2);
     TORCH_CHECK(eps >= 0, op, ": eps is not negative, got ", eps);
@@ -1262,7 +1266,7 @@ void adamw_multi(const char* op, const TensorList& params, const TensorList& exp
     GSX_DEVICE_GUARD(params[0]);
     const at::Device dev = params[0].device();
     const double* ctl = control_of(control, dev, op);
-    TORCH_CHECK(!steps.empty() || ctl != nullptr, op, ": steps may be empty only with a control block");
+    TORCH_CHECK(!steps.v.empty() || ctl != nullptr, op, ": steps may be empty only with a control block");
     TORCH_CHECK(!seed.has_value() || (*seed >= 0 && *seed <= 0xFFFFFFFFll), op, ": seed lies in 0 .. 2^32 - 1");
     std::vector<gsx_adamw_tensor> list(k);
     std::vector<const void*> written;
@@ -1281,10 +1285,10 @@ void adamw_multi(const char* op, const TensorList& params, const TensorList& exp
         uint64_t rp, cp, rg, cg;
         rows_of(p, rp, cp, x.ld_param, op, "parameter", i);
         rows_of(g, rg, cg, x.ld_grad, op, "gradient", i);
-        const auto split = splits.empty() ? std::make_tuple((int64_t)0, 0.0, 0.0, false, false) : splits[i];
+        const Split split = splits.v.empty() ? Split{} : splits.v[i];
         // a dense tensor counts as one row unless something goes by rows: the other of the two, or the column groups
         x.rows = rp; x.cols = cp;
-        const bool groups = std::get<0>(split) != 0;
+        const bool groups = split.split != 0;
         if (p.numel() != 0 && (rp != rg || cp != cg || groups)) {
             TORCH_CHECK(p.dim() >= 1, op, ": a split needs rows");
             x.rows = (uint64_t)p.size(0); x.cols = (uint64_t)(p.numel() / p.size(0));
@@ -1292,7 +1296,7 @@ void adamw_multi(const char* op, const TensorList& params, const TensorList& exp
             if (rg == 1 && cg == (uint64_t)g.numel()) x.ld_grad = x.cols;
         }
         if (groups)
-            TORCH_CHECK(std::get<0>(split) > 0 && (p.numel() == 0 || (uint64_t)std::get<0>(split) <= x.cols), op, ": split ", std::get<0>(split), " of parameter ", i,
+            TORCH_CHECK(split.split > 0 && (p.numel() == 0 || (uint64_t)split.split <= x.cols), op, ": split ", split.split, " of parameter ", i,
                         " lies beyond its ", x.cols, " columns");
         x.param = p.data_ptr(); x.grad = g.data_ptr(); x.exp_avg = m.data_ptr(); x.exp_avg_sq = v.data_ptr();
         if (eight) {
@@ -1304,12 +1308,12 @@ void adamw_multi(const char* op, const TensorList& params, const TensorList& exp
             }
             x.avg_scale = avg_scales[i].data_ptr<float>(); x.rms_scale = rms_scales[i].data_ptr<float>();
         }
-        x.split = (uint32_t)std::get<0>(split); x.lr_b = (float)std::get<1>(split); x.weight_decay_b = (float)std::get<2>(split);
-        x.hold = std::get<3>(split); x.hold_b = std::get<4>(split);
-        x.lr = (float)lrs[i]; x.weight_decay = (float)weight_decays[i];
-        if (!steps.empty()) {
-            TORCH_CHECK(steps[i] >= 1 && steps[i] <= 0xFFFFFFFFll, op, ": steps count from 1, got ", steps[i], " for parameter ", i);
-            x.step = (uint64_t)steps[i];
+        x.split = (uint32_t)split.split; x.lr_b = (float)split.lr_b; x.weight_decay_b = (float)split.weight_decay_b;
+        x.hold = split.hold_a; x.hold_b = split.hold_b;
+        x.lr = (float)lrs.v[i]; x.weight_decay = (float)weight_decays.v[i];
+        if (!steps.v.empty()) {
+            TORCH_CHECK(steps.v[i] >= 1 && steps.v[i] <= 0xFFFFFFFFll, op, ": steps count from 1, got ", steps.v[i], " for parameter ", i);
+            x.step = (uint64_t)steps.v[i];
         }
         if (p.numel() != 0) written.insert(written.end(), {x.param, x.exp_avg, x.exp_avg_sq});
     }
@@ -1321,14 +1325,14 @@ void adamw_multi(const char* op, const TensorList& params, const TensorList& exp
 }  // namespace
 
 void adamw_step_multi(const TensorList& params, const TensorList& exp_avgs, const TensorList& exp_avg_sqs, const TensorList& grads,
-                      const std::vector<double>& lrs, const std::vector<double>& weight_decays, double beta1, double beta2, double eps, const std::vector<int64_t>& steps,
+                      const Numbers& lrs, const Numbers& weight_decays, double beta1, double beta2, double eps, const Counts& steps,
                       at::optional<at::Tensor> control, const Splits& splits) {
     adamw_multi("adamw_step_multi", params, exp_avgs, exp_avg_sqs, {}, {}, false, grads, lrs, weight_decays, beta1, beta2, eps, steps, control, splits, at::nullopt);
 }
 
 void adamw8_step_multi(const TensorList& params, const TensorList& exp_avgs, const TensorList& exp_rmss, const TensorList& avg_scales,
-                       const TensorList& rms_scales, const TensorList& grads, const std::vector<double>& lrs, const std::vector<double>& weight_decays,
-                       double beta1, double beta2, double eps, const std::vector<int64_t>& steps, at::optional<at::Tensor> control, const Splits& splits,
+                       const TensorList& rms_scales, const TensorList& grads, const Numbers& lrs, const Numbers& weight_decays,
+                       double beta1, double beta2, double eps, const Counts& steps, at::optional<at::Tensor> control, const Splits& splits,
                        at::optional<int64_t> seed) {
     adamw_multi("adamw8_step_multi", params, exp_avgs, exp_rmss, avg_scales, rms_scales, true, grads, lrs, weight_decays, beta1, beta2, eps, steps, control, splits, seed);
 }
@@ -1453,6 +1457,58 @@ template <> struct type_caster<gsx_ext::TensorList> {
             PyObject* o = PySequence_Fast_GET_ITEM(src.ptr(), i);
             if (!THPVariable_Check(o)) return false;
             value.t[(size_t)i] = &THPVariable_Unpack(o);
+        }
+        return true;
+    }
+};
+// Python numbers (whatever has __float__ or __index__); false, with no error left behind, for anything else.
+inline bool read_number(PyObject* o, double* v) {
+    *v = PyFloat_CheckExact(o) ? PyFloat_AS_DOUBLE(o) : PyFloat_AsDouble(o);
+    if (*v == -1.0 && PyErr_Occurred()) { PyErr_Clear(); return false; }
+    return true;
+}
+inline bool read_count(PyObject* o, int64_t* v) {
+    if (PyFloat_Check(o)) return false;
+    *v = PyLong_AsLongLong(o);
+    if (*v == -1 && PyErr_Occurred()) { PyErr_Clear(); return false; }
+    return true;
+}
+inline bool is_sequence(PyObject* o) { return PyList_Check(o) || PyTuple_Check(o); }
+template <> struct type_caster<gsx_ext::Numbers> {
+    PYBIND11_TYPE_CASTER(gsx_ext::Numbers, const_name("list[float]"));
+    bool load(handle src, bool) {
+        if (!is_sequence(src.ptr())) return false;
+        value.v.resize((size_t)PySequence_Fast_GET_SIZE(src.ptr()));
+        for (size_t i = 0; i < value.v.size(); ++i)
+            if (!read_number(PySequence_Fast_GET_ITEM(src.ptr(), (Py_ssize_t)i), &value.v[i])) return false;
+        return true;
+    }
+};
+template <> struct type_caster<gsx_ext::Counts> {
+    PYBIND11_TYPE_CASTER(gsx_ext::Counts, const_name("list[int]"));
+    bool load(handle src, bool) {
+        if (!is_sequence(src.ptr())) return false;
+        value.v.resize((size_t)PySequence_Fast_GET_SIZE(src.ptr()));
+        for (size_t i = 0; i < value.v.size(); ++i)
+            if (!read_count(PySequence_Fast_GET_ITEM(src.ptr(), (Py_ssize_t)i), &value.v[i])) return false;
+        return true;
+    }
+};
+template <> struct type_caster<gsx_ext::Splits> {
+    PYBIND11_TYPE_CASTER(gsx_ext::Splits, const_name("list[tuple[int, float, float, bool, bool]]"));
+    bool load(handle src, bool) {
+        if (!is_sequence(src.ptr())) return false;
+        value.v.resize((size_t)PySequence_Fast_GET_SIZE(src.ptr()));
+        for (size_t i = 0; i < value.v.size(); ++i) {
+            PyObject* o = PySequence_Fast_GET_ITEM(src.ptr(), (Py_ssize_t)i);
+            if (!is_sequence(o) || PySequence_Fast_GET_SIZE(o) != 5) return false;
+            gsx_ext::Split& x = value.v[i];
+            const int a = PyObject_IsTrue(PySequence_Fast_GET_ITEM(o, 3)), b = PyObject_IsTrue(PySequence_Fast_GET_ITEM(o, 4));
+            if (a < 0 || b < 0) { PyErr_Clear(); return false; }
+            x.hold_a = a != 0; x.hold_b = b != 0;
+            if (!read_count(PySequence_Fast_GET_ITEM(o, 0), &x.split) || !read_number(PySequence_Fast_GET_ITEM(o, 1), &x.lr_b) ||
+                !read_number(PySequence_Fast_GET_ITEM(o, 2), &x.weight_decay_b))
+                return false;
         }
         return true;
     }
@@ -1618,10 +1674,10 @@ PYBIND11_MODULE(_gsx_ops, m) {
     m.attr("CONTROL_WORDS") = GSX_CONTROL_WORDS;
     m.def("adamw_step_multi", &gsx_ext::adamw_step_multi, py::arg("params"), py::arg("exp_avgs"), py::arg("exp_avg_sqs"), py::arg("grads"), py::arg("lrs"),
           py::arg("weight_decays"), py::arg("beta1"), py::arg("beta2"), py::arg("eps"), py::arg("steps"), py::arg("control") = py::none(),
-          py::arg("splits") = gsx_ext::Splits());
+          py::arg("splits") = py::tuple());
     m.def("adamw8_step_multi", &gsx_ext::adamw8_step_multi, py::arg("params"), py::arg("exp_avgs"), py::arg("exp_rmss"), py::arg("avg_scales"),
           py::arg("rms_scales"), py::arg("grads"), py::arg("lrs"), py::arg("weight_decays"), py::arg("beta1"), py::arg("beta2"), py::arg("eps"),
-          py::arg("steps"), py::arg("control") = py::none(), py::arg("splits") = gsx_ext::Splits(), py::arg("seed") = py::none());
+          py::arg("steps"), py::arg("control") = py::none(), py::arg("splits") = py::tuple(), py::arg("seed") = py::none());
     m.def("grad_norm_multi", &gsx_ext::grad_norm_multi, py::arg("grads"), py::arg("control"), py::arg("max_norm") = std::numeric_limits<double>::infinity());
     m.def("adamw8_select_rows", &gsx_ext::adamw8_select_rows, py::arg("exp_avgs"), py::arg("exp_rmss"), py::arg("avg_scales"), py::arg("rms_scales"),
           py::arg("index"));
