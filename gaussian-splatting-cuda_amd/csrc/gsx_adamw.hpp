@@ -49,7 +49,7 @@ template <class R, uint32_t L> struct Chunks {
     uint32_t chunks, per;   // of the launch; of a workgroup
 };
 
-// Walks this workgroup's chunks: tensor(rec) for every tensor among them, then chunk(index within the tensor) for each of its chunks.
+// Walks this workgroup's chunks: tensor(rec, first, stop) for every tensor among them, first and stop counted within the tensor.
 template <class R, uint32_t L, class T> GSX_DEV void walk(const Chunks<R, L>& a, T tensor) {
     uint32_t begin[(L + 63) / 64];
     const uint32_t lane = threadIdx.x & 63u;

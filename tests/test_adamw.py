@@ -61,6 +61,7 @@ def test_adamw_entry_points_refuse_bad_tensors(bad):
 
 def test_adamw_entry_points_refuse_bad_scalars_and_take_empty_lists():
     l, d = lib(), ctypes.c_double
+    assert l.gsx_optim_abi_version() == 1   # include/gsx_optim.h GSX_OPTIM_ABI_VERSION
     for f, more in ((l.gsx_adamw_step_multi, ()), (l.gsx_adamw8_step_multi, (ctypes.c_int(0), ctypes.c_uint32(0)))):
         for b1, b2, eps in ((1.0, 0.9, 0.0), (-0.1, 0.9, 0.0), (0.9, 1.0, 0.0), (float("nan"), 0.9, 0.0), (0.9, 0.99, -1e-8), (0.9, 0.99, float("nan"))):
             assert f(ctypes.c_uint32(1), (Tensor * 1)(good()), d(b1), d(b2), d(eps), *more, None, None) == -1
