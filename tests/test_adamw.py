@@ -937,3 +937,28 @@ def test_captured_steps_of_a_long_list():
         for name in ("p", "m", "v"):
             assert all(torch.equal(a, b) for a, b in zip(eager[name], captured[name])), (it, name)
         assert torch.equal(eager["c"], captured["c"])
+
+
+@pytest.mark.gpu
+def test_fused_adamw_by_rows_equals_the_whole_step():
+    """step(rows=...) on two copies, each with its block of rows: together the bits of one step over all rows (distributed.ShardedAdam's use)."""
+    import gsx  # noqa: F401
+    from gsx import optim
+    n, cut = 401, 170
+    models = [splat_model(n, 16, "cuda") for _ in range(3)]
+    opts = [optim.FusedAdamW.for_splat_data(m, weight_decay={"shN": 0.2, "rotation": 0.1}) for m in models]
+    for t in range(3):
+        g = [torch.randn(p.shape, generator=torch.Generator().manual_seed(10 * t + i)).cuda() for i, p in enumerate(models[0].params())]
+        for m in models:
+            for p, x in zip(m.params(), g):
+                p.grad = x.clone()
+        it = 999 + t   # shN held, held, stepped
+        opts[0].step(it)
+        opts[1].step(it, rows=(0, cut))
+        opts[2].step(it, rows=(cut, n))
+        for whole, lo, hi in zip(*(m.params() for m in models)):
+            assert torch.equal(whole[:cut], lo[:cut]) and torch.equal(whole[cut:], hi[cut:])
+    for k, st in opts[0].state.items():
+        for name in ("exp_avg", "exp_avg_sq"):
+            assert torch.equal(st[name][:cut], opts[1].state[k][name][:cut]) and bool((opts[1].state[k][name][cut:] == 0).all())
+            assert torch.equal(st[name][cut:], opts[2].state[k][name][cut:])
