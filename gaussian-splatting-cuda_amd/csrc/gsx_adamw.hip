@@ -183,7 +183,7 @@ template <class F> int norm_lists(uint32_t count, const gsx_grad_tensor* tensors
     for (uint32_t i = 0; i < count; ++i) mask |= 1u << tensors[i].dtype;
     for (uint32_t d = 0; d <= GSX_DTYPE_F16; ++d) {
         if (!(mask >> d & 1u)) continue;
-        const int rc = launch_lists<NormList, NormRec>(
+        const int rc = launch_lists<NormList>(
             count, kNormChunk, [](uint32_t chunks) { return (chunks + kNormGrid - 1) / kNormGrid; },
             [&](uint32_t i, NormRec* r, uint64_t* n) {
                 const gsx_grad_tensor& x = tensors[i];
@@ -276,7 +276,7 @@ extern "C" int gsx_adamw_step_multi(uint32_t count, const gsx_adamw_tensor* tens
     for (uint32_t types = 0; types < 9; ++types) {
         if (!(mask >> types & 1u)) continue;
         const uint32_t pd = types / 3, gd = types % 3;
-        const int rc = launch_lists<List, Rec>(
+        const int rc = launch_lists<List>(
             count, kChunk, [](uint32_t) { return kPer; },
             [&](uint32_t i, Rec* r, uint64_t* n) {
                 if (tensors[i].param_dtype != pd || tensors[i].grad_dtype != gd) return false;

@@ -80,39 +80,34 @@ inline bool count_of(uint64_t rows, uint64_t cols, uint64_t* n) {
 
 // Gathers tensors and launches them: item(i, &rec, &values) is false for a tensor that does not belong here; launch(args, workgroups) for every full list, args an
 // Args<L> (with its tensors in args.c) whose other members are the launch's to fill.  per(chunks): how many of them a workgroup takes.
-template <template <uint32_t> class Args, class R, class Per, class Item, class Launch>
-int launch_lists(uint32_t count, uint32_t chunk, Per per, Item item, Launch launch) {
-    R rec[kMany];
-    uint32_t begin[kMany];
+template <uint32_t L, template <uint32_t> class Args, class Per, class Item, class Launch>
+int launch_lists_of(uint32_t count, uint32_t chunk, Per per, Item item, Launch launch) {
+    Args<L> a;
     uint32_t i = 0;
     while (i < count) {
         uint32_t k = 0;
         uint64_t chunks = 0;
-        for (; i < count; ++i) {
+        for (; i < count && k < L; ++i) {
             uint64_t n = 0;
-            R r;
-            if (!item(i, &r, &n) || n == 0) continue;
-            if (k == kMany || (k != 0 && chunks + chunks_of(n, chunk) > kMostChunks)) break;
-            rec[k] = r;
-            begin[k++] = (uint32_t)chunks;
+            if (!item(i, &a.c.rec[k], &n) || n == 0) continue;
+            if (k != 0 && chunks + chunks_of(n, chunk) > kMostChunks) break;
+            a.c.begin[k++] = (uint32_t)chunks;
             chunks += chunks_of(n, chunk);
         }
         if (k == 0) break;
-        auto go = [&](auto room) {
-            constexpr uint32_t L = decltype(room)::value;
-            Args<L> a;
-            std::copy_n(rec, k, a.c.rec);
-            std::copy_n(begin, k, a.c.begin);
-            std::fill(a.c.begin + k, a.c.begin + L + 1, 0xFFFFFFFFu);
-            a.c.chunks = (uint32_t)chunks;
-            a.c.per = std::max(per(a.c.chunks), (a.c.chunks + kMostBlocks - 1) / kMostBlocks);
-            return launch(a, (a.c.chunks + a.c.per - 1) / a.c.per);
-        };
-        const int rc = k <= kFew ? go(std::integral_constant<uint32_t, kFew>{}) : k <= kSome ? go(std::integral_constant<uint32_t, kSome>{})
-                                                                                            : go(std::integral_constant<uint32_t, kMany>{});
+        std::fill(a.c.begin + k, a.c.begin + L + 1, 0xFFFFFFFFu);
+        a.c.chunks = (uint32_t)chunks;
+        a.c.per = std::max(per(a.c.chunks), (a.c.chunks + kMostBlocks - 1) / kMostBlocks);
+        const int rc = launch(a, (a.c.chunks + a.c.per - 1) / a.c.per);
         if (rc != GSX_OK) return rc;
     }
     return GSX_OK;
+}
+template <template <uint32_t> class Args, class Per, class Item, class Launch>
+int launch_lists(uint32_t count, uint32_t chunk, Per per, Item item, Launch launch) {
+    if (count <= kFew) return launch_lists_of<kFew, Args>(count, chunk, per, item, launch);
+    if (count <= kSome) return launch_lists_of<kSome, Args>(count, chunk, per, item, launch);
+    return launch_lists_of<kMany, Args>(count, chunk, per, item, launch);
 }
 
 // Launches a kernel whose one argument is a list, from where the list lies (the launch expression would copy its 2 to 32 KB once more).

@@ -379,7 +379,7 @@ extern "C" int gsx_adamw8_step_multi(uint32_t count, const gsx_adamw_tensor* ten
     for (uint32_t types = 0; types < 9; ++types) {
         if (!(mask >> types & 1u)) continue;
         const uint32_t pd = types / 3, gd = types % 3;
-        const int rc = launch_lists<List, Rec>(
+        const int rc = launch_lists<List>(
             count, kChunk, per_of,
             [&](uint32_t i, Rec* r, uint64_t* n) {
                 if (tensors[i].param_dtype != pd || tensors[i].grad_dtype != gd) return false;
@@ -418,7 +418,7 @@ extern "C" int gsx_adamw8_select_rows(uint32_t count, const gsx_moments8* tensor
         if (!x.avg_out || !x.rms_out || !x.avg_scale_out || !x.rms_scale_out) return invalid("adamw8_select_rows: null tensor");
         if (rows_in != 0 && (!x.avg_in || !x.rms_in || !x.avg_scale_in || !x.rms_scale_in)) return invalid("adamw8_select_rows: null tensor");
     }
-    return launch_lists<SelectList, SelectRec>(
+    return launch_lists<SelectList>(
         count, kSelect, [](uint32_t) { return 1u; },
         [&](uint32_t i, SelectRec* r, uint64_t* n) {
             const gsx_moments8& x = tensors[i];
