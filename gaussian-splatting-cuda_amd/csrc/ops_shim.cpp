@@ -1249,7 +1249,6 @@ bool repeats(const std::vector<const void*>& addresses) {
     return false;
 }
 
-
 // What both AdamW operators share; `scales` is empty for moments in 32 bits.
 void adamw_multi(const char* op, const TensorList& params, const TensorList& exp_avgs, const TensorList& exp_avg_sqs,
                  const TensorList& avg_scales, const TensorList& rms_scales, bool eight, const TensorList& grads,
