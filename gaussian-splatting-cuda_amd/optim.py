@@ -254,11 +254,16 @@ class FusedAdamW(FusedAdam):
     def step_count(self, name):
         return self.steps
 
+    def _outcome(self):
+        if self.control is None:
+            raise RuntimeError("FusedAdamW: the norm and the skip flag are those of a step with max_grad_norm, and there has been none")
+        return self.control
+
     def last_norm(self):
-        return float(self.control[0])
+        return float(self._outcome()[0])
 
     def skipped_last(self):
-        return bool(self.control[2])
+        return bool(self._outcome()[2])
 
     def reset_state(self, indices):
         if self.moments == 32:

@@ -962,3 +962,13 @@ def test_fused_adamw_by_rows_equals_the_whole_step():
         for name in ("exp_avg", "exp_avg_sq"):
             assert torch.equal(st[name][:cut], opts[1].state[k][name][:cut]) and bool((opts[1].state[k][name][cut:] == 0).all())
             assert torch.equal(st[name][cut:], opts[2].state[k][name][cut:])
+
+
+def test_fused_adamw_has_no_norm_before_a_clipped_step():
+    import gsx  # noqa: F401
+    from gsx import optim
+    for options in ({}, {"max_grad_norm": 1.0}):
+        opt = optim.FusedAdamW.for_splat_data(splat_model(5, 1, "cpu"), **options)
+        for read in (opt.last_norm, opt.skipped_last):
+            with pytest.raises(RuntimeError, match="max_grad_norm"):
+                read()
