@@ -63,8 +63,11 @@ def build_libgsx(force=False, verbose=False):
         objs.append(o)
         # -fno-slp-vectorize: v_pk_fma_f32 / v_pk_mul_f32 issue at ~7.5 cycles per wave64 instruction on gfx950 vs ~2.9 for the
         # scalar forms (tools/valu_probe.hip), so SLP-packed fp32 math is a net loss in the VALU-bound blend loops
-        # -packed-fp32-ops: no packed fp32 instructions at all, also where the compiler would make them without SLP (the host pass says that it does not
-        # know the feature: harmless).  The blend kernels' code is the same with and without it (they held none): blend_kernel_hash() leaves it out.
+        # -packed-fp32-ops: no packed fp32 instructions at all, whatever the compiler would make of a source (the host pass says that it does not know the
+        # feature: harmless).  No source holds any either way (tests/test_build.py reads the library); what the flag changes is that the compiler no longer opens loops
+        # by two or four: in gsx_sh.hip, gsx_intersect.hip and gsx_adamw8.hip, the others compile to the same code (so blend_kernel_hash() leaves it out).  With / without
+        # it on one box, 1 M splats, us: sh_colors_bwd 209.7 / 210.6, sh_fwd 62.5 / 62.5, sh_bwd 73.6 / 74.4, bin_count 11.6 / 11.8, bin_prefix_scan 10.6 / 9.9,
+        # bin_scatter 28.1 / 28.4 (5 M: 232 / 234, opened in the source), tile_sort 30.1 / 30.4, rs_scatter 16.1 / 16.0; a training iteration the same.
         cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-slp-vectorize", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + \
             os.environ.get("GSX_EXTRA_HIPCC_FLAGS", "").split() + ["-c", s, "-o", o]  # (tuning experiments: -DGSX_FCH=..., ...)
         procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))

@@ -308,6 +308,8 @@ __global__ __launch_bounds__(BIN_BLOCK) void bin_scatter_kernel(uint32_t N, uint
     const uint32_t n_tiles = tw * th, c = blockIdx.y, b = blockIdx.x;
     const uint32_t* pre = block_hist + ((size_t)c * BIN_NB + b) * n_tiles;
     const int32_t* off = tile_offsets + (size_t)c * n_tiles;
+    // (four tiles' loads in flight: 5 M splats 232 us, one after the other 239)
+#pragma unroll 4
     for (uint32_t t = threadIdx.x; t < n_tiles; t += BIN_BLOCK) s_cur[t] = (uint32_t)off[t] + pre[t];
     __syncthreads();
     (void)per_block;
