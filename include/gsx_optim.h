@@ -65,7 +65,8 @@ int gsx_adamw_step_multi(uint32_t count, const gsx_adamw_tensor* tensors, double
 /* The same with m and r = sqrt(v) stored as OCP e4m3 numbers, one scale for each GSX_MOMENT_RUN consecutive values (the last run of a tensor may be
  * shorter): scale = max(largest finite |x| of the run * (1 / 448 in 32 bits), 2^-120), code = x / scale rounded; infinities and NaN become NaN; an r above zero is
  * never stored as zero.  Zero codes (with any finite scale) are zero moments.  The moments are formed product by product and sum by sum, each rounded to 32
- * bits ((1 - beta2) g times g), so that the codes are a function of the inputs to the last bit.
+ * bits ((1 - beta2) g times g), the root and the quotient x / scale too, so that the codes are a function of the inputs to the last bit (but for scales between 2^-120 and 2^-93,
+ * where the quotient may be off by one place of its 24 bits).
  * stochastic 0: to the nearest code, ties to even.  Else to one of the two neighbours: away from zero if (the part of the step between them) + u >= 1,
  * u the high (m) or low (r) 16 bits of mix(i + key) / 2^16 for value i of the tensor, i taken modulo 2^32,
  *   key = mix(mix(seed + 0x9E3779B9 t) + 0xC2A6F0B5 k) + 0x61C8864F floor(i / 2^32) for tensor k of the list, all in 32 bits,

@@ -1,0 +1,88 @@
+"""The optimizer operators over many tensors (include/gsx_optim.h) at their edges: quotients next to the middle between two numbers, runs of chunks that cross from tensor
+to tensor, views with 8-bit moments, what is refused, what autograd is told — against the plain forms in 64 bits (adamw_reference.py)."""
+import pytest
+import torch
+
+from tests import adamw_reference as ref
+
+f8 = torch.float8_e4m3fn
+
+
+def quotients_next_to_the_middle(count, seed):
+    """float32 pairs (x, s), 1 <= x / s < 2, whose quotient is (Q + 1/2 +- 1 / (2 S)) 2^-23, S the significand of s: no quotient of two such numbers lies nearer to the
+    middle between its neighbours Q and Q + 1.  (X 2^24 = (2 Q + 1) S +- 1, so 2 Q + 1 is -+ the inverse of S modulo 2^24.)  Q + 1 is a multiple of 16: one of
+    the two neighbours lies on a border of the stochastic rounding."""
+    gen = torch.Generator().manual_seed(seed)
+    S = (torch.randint(2 ** 22, 2 ** 23, (64 * count,), generator=gen) * 2 + 1).unique()
+    inverse = S.clone()
+    for _ in range(5):
+        inverse = inverse * ((2 - S * inverse) % 2 ** 24) % 2 ** 24
+    X, D = [], []
+    for r in (1, -1):
+        q = (-r * inverse) % 2 ** 24 + 2 ** 24
+        num = q * S + r
+        x = num >> 24
+        ok = (num % 2 ** 24 == 0) & (x >= S) & (x < 2 ** 24) & ((q + 1) % 32 == 0)
+        X.append(x[ok])
+        D.append(S[ok])
+    X, D = torch.cat(X), torch.cat(D)
+    pick = torch.randperm(X.numel(), generator=gen)[:count]
+    assert pick.numel() == count
+    return X[pick].float() * 2.0 ** -40, D[pick].float() * 2.0 ** -40   # (24 bits each: exact)
+
+
+def largest_of_scale(s):
+    """float32 values t with t * (1 / 448) = s in 32 bits, NaN where there is none."""
+    c, out = torch.tensor(1.0 / 448.0, dtype=torch.float32), torch.full_like(s, float("nan"))
+    near = (s.double() * 448).float().view(torch.int32)
+    for d in range(-2, 3):
+        t = (near + d).view(torch.float32)
+        out = torch.where(t * c == s, t, out)
+    return out
+
+
+@pytest.mark.gpu
+def test_codes_of_quotients_next_to_the_middle():
+    """x / scale is rounded to the nearest float32 before it becomes a code: 20 000 of the hardest quotients, each at a place whose draw decides by the last bit of the
+    quotient.  beta1 = 0 makes the first moment the gradient itself."""
+    import gsx  # noqa: F401
+    from gsx import ops
+    runs, seed, step = 65536, 5, 9
+    n = runs * 128
+    x, s = quotients_next_to_the_middle(26000, 1)
+    t = largest_of_scale(s)
+    x, s, t = x[~t.isnan()][:20000], s[~t.isnan()][:20000], t[~t.isnan()][:20000]
+    assert x.numel() == 20000
+    y = (x.double() / s.double()).float()        # (a double is never as near to a middle as these are far from it: 2^-25 of a place)
+    u = ref.draws(seed, step, 0, 0, n)[0]
+    word = (u * 65536).long()
+    word[127::128] = -1                          # the last place of a run holds its largest value
+    border = (x.double() / s.double() * 2 ** 23).round().long()
+    border = torch.where(border % 16 == 0, border, border + 1)     # Q + 1
+    need = (-(border % 2 ** 20) % 2 ** 20) // 16                   # the draw that carries from there, and not from Q
+    order = word.argsort()
+    at = torch.searchsorted(word[order], need).tolist()
+    places, used, kept = [], set(), []
+    order, need = order.tolist(), need.tolist()
+    for k in range(len(need)):
+        i = at[k]
+        while i < n and int(word[order[i]]) == need[k] and order[i] // 128 in used:
+            i += 1
+        if i < n and int(word[order[i]]) == need[k]:
+            used.add(order[i] // 128)
+            places.append(order[i])
+            kept.append(k)
+    assert len(kept) > 19000
+    places, kept = torch.tensor(places), torch.tensor(kept)
+    x, s, t, y = x[kept], s[kept], t[kept], y[kept]
+    sign = torch.where(torch.arange(len(kept)) % 2 == 0, 1.0, -1.0)
+    g = torch.zeros(n)
+    g[places] = x * sign
+    g[places // 128 * 128 + 127] = t
+    m, r = (torch.zeros(n, dtype=torch.uint8, device="cuda").view(f8) for _ in range(2))
+    sm, sr = torch.zeros(runs, device="cuda"), torch.zeros(runs, device="cuda")
+    ops.adamw8_step_multi([torch.zeros(n, device="cuda")], [m], [r], [sm], [sr], [g.cuda()], [0.0], [0.0], 0.0, 0.999, 1e-8, [step], seed=seed)
+    assert torch.equal(sm.cpu()[places // 128], s)
+    want = ref.rounded(y.double(), False, u[places]) * sign
+    got = m.cpu()[places].double()
+    assert torch.equal(got, want.double()), "%d of %d codes" % (int((got != want).sum()), len(kept))
