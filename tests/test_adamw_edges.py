@@ -86,3 +86,54 @@ def test_codes_of_quotients_next_to_the_middle():
     want = ref.rounded(y.double(), False, u[places]) * sign
     got = m.cpu()[places].double()
     assert torch.equal(got, want.double()), "%d of %d codes" % (int((got != want).sum()), len(kept))
+
+
+# ---- what is refused -----------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_a_scale_twice_in_the_lists_is_refused():
+    """One scale tensor for both moments, for two parameters, or in the place of another tensor: the runs would overwrite each other's."""
+    import gsx  # noqa: F401
+    from gsx import ops
+    z = lambda *s, dt=torch.float32: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+    p, m, r = [z(200), z(200)], [z(200, dt=f8), z(200, dt=f8)], [z(200, dt=f8), z(200, dt=f8)]
+    call = lambda sm, sr, p=p: ops.adamw8_step_multi(p, m, r, sm, sr, [z(200)] * 2, [0.1] * 2, [0.0] * 2, 0.9, 0.999, 1e-8, [1, 1])  # noqa: E731
+    a, b, c, d = (z(2) for _ in range(4))
+    call([a, b], [c, d])
+    for sm, sr in (([a, b], [a, d]), ([a, a], [c, d]), ([a, b], [c, c]), ([a, b], [c, a])):
+        with pytest.raises(RuntimeError, match="twice"):
+            call(sm, sr)
+    with pytest.raises(RuntimeError, match="twice"):
+        call([p[1][:2], b], [c, d])
+    e = z(0)                                     # (empty tensors have no memory to share)
+    ops.adamw8_step_multi([e, e], [z(0, dt=f8)] * 2, [z(0, dt=f8)] * 2, [e, e], [e, e], [e, e], [0.1] * 2, [0.0] * 2, 0.9, 0.999, 1e-8, [1, 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [1, 2, 40])
+def test_a_tensor_twice_is_found_wherever_it_is(count):
+    """Lists cut one behind the other from flat buffers (seen to be apart by their order) and in any other order (by a table): taken as they are, refused with any
+    tensor of theirs in the place of another."""
+    import gsx  # noqa: F401
+    from gsx import ops
+    gen = torch.Generator().manual_seed(count)
+
+    def lists(ascending):
+        flat = [torch.zeros(200 * count, device="cuda"), torch.zeros(200 * count, dtype=f8, device="cuda"), torch.zeros(200 * count, dtype=f8, device="cuda"),
+                torch.zeros(2 * count, device="cuda"), torch.zeros(2 * count, device="cuda")]
+        cut = [list(t.split(t.numel() // count)) for t in flat]
+        if not ascending:
+            cut = [[c[i] for i in torch.randperm(count, generator=gen).tolist()] for c in cut]
+        return cut
+    def call(x):
+        ops.adamw8_step_multi(*x[:3], x[3], x[4], [torch.zeros(200, device="cuda")] * count, [0.1] * count, [0.0] * count, 0.9, 0.999, 1e-8, [1] * count)
+    for ascending in (True, False):
+        call(lists(ascending))
+        for a in range(5):
+            for b in range(5):
+                i, j = (int(k) for k in torch.randint(0, count, (2,), generator=gen))
+                if (a in (1, 2)) != (b in (1, 2)) or (a == 0) != (b == 0) or (a == b and i == j):
+                    continue   # (of another type or size: refused for that)
+                x = lists(ascending)
+                x[a][i] = x[b][j]
+                with pytest.raises(RuntimeError, match="twice"):
+                    call(x)
