@@ -1223,8 +1223,9 @@ void rows_of(const at::Tensor& t, uint64_t& rows, uint64_t& cols, uint64_t& ld, 
     TORCH_CHECK(t.stride(0) >= inner, op, ": ", what, " ", i, " has rows that overlap (sizes ", t.sizes(), ", strides ", t.strides(), "): make it contiguous");
 }
 
+// (dev: the guarded tensor's, a GPU's)
 void check_on(const at::Tensor& t, const at::Device& dev, const char* op, const char* what, size_t i) {
-    TORCH_CHECK(t.is_cuda() && t.device() == dev, op, ": ", what, " ", i, " is on ", t.device(), ", the first tensor on ", dev);
+    TORCH_CHECK(t.device() == dev, op, ": ", what, " ", i, " is on ", t.device(), ", the first tensor on ", dev);
 }
 
 const double* control_of(const at::optional<at::Tensor>& control, const at::Device& dev, const char* op) {
@@ -1328,6 +1329,8 @@ void adamw_multi(const char* op, const TensorList& params, const TensorList& exp
     TORCH_CHECK(!repeats(written, eight ? 5 : 3), op, ": a parameter, a moment or a scale is in the lists twice");
     if (eight) check(gsx_adamw8_step_multi((uint32_t)k, list.data(), beta1, beta2, eps, seed.has_value(), (uint32_t)seed.value_or(0), ctl, cur_stream()), op);
     else check(gsx_adamw_step_multi((uint32_t)k, list.data(), beta1, beta2, eps, ctl, cur_stream()), op);
+    for (size_t i = 0; i < k; ++i)   // autograd refuses a backward that would read a parameter's old values (as behind any in-place operation; the moments are in no graph)
+        if (!params[i].is_inference()) params[i].unsafeGetTensorImpl()->bump_version();
 }
 
 }  // namespace

@@ -89,7 +89,8 @@ def grad_norm_multi(grads, control, max_norm=float("inf")):
 
 def adamw_step_multi(params, exp_avgs, exp_avg_sqs, grads, lrs, weight_decays, beta1, beta2, eps, steps, control=None, splits=()):
     """AdamW with decoupled decay on every tensor of the lists, in place: moments contiguous float32, a rate and a decay for each tensor.  16-bit parameters are rounded to
-    nearest after the step (a step below half a place of theirs leaves them where they are).  No two tensors of the lists may share memory.
+    nearest after the step (a step below half a place of theirs leaves them where they are).  No two tensors of the lists may share memory.  The parameters' version
+    counters advance: a backward through a graph from before the step that needs their old values is refused, as behind the library's own optimizers.
     steps: the number of this step for each tensor, from 1; empty: the control block's.  control (step_control): the gradients are multiplied by its factor,
     and nothing is changed where its skip flag is set.  splits, one for each tensor or empty: (split, lr_b, weight_decay_b, hold_a, hold_b) — the columns
     [split, ...) of a tensor seen as rows are a second group with its own rate and decay (0: one group); a held group and its moments stay as they are."""

@@ -328,10 +328,10 @@ class FusedAdamW(FusedAdam):
         col = lambda k: [r(st[k]) for st in sts]  # noqa: E731
         control = self.control if not steps else None
         if self.moments == 32:
-            ops.adamw_step_multi([r(p.data) for p in params], col("exp_avg"), col("exp_avg_sq"), grads, *args, control=control, splits=splits)
+            ops.adamw_step_multi([r(p) for p in params], col("exp_avg"), col("exp_avg_sq"), grads, *args, control=control, splits=splits)
         else:
             whole = lambda k: [st[k] for st in sts]  # noqa: E731
-            ops.adamw8_step_multi([p.data for p in params], whole("exp_avg"), whole("exp_rms"), whole("avg_scale"), whole("rms_scale"), grads, *args,
+            ops.adamw8_step_multi(params, whole("exp_avg"), whole("exp_rms"), whole("avg_scale"), whole("rms_scale"), grads, *args,
                                   control=control, splits=splits, seed=self.seed)
 
 

@@ -137,3 +137,44 @@ def test_a_tensor_twice_is_found_wherever_it_is(count):
                 x[a][i] = x[b][j]
                 with pytest.raises(RuntimeError, match="twice"):
                     call(x)
+
+
+# ---- what autograd is told -------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_backward_over_a_step_is_refused(bits):
+    """A graph kept over a step that needs a parameter's old values: an error, not gradients of the new ones.  Through the operators and through the optimizer."""
+    import gsx  # noqa: F401
+    from gsx import ops, optim
+    from tests.test_adamw import splat_model
+    z = lambda *s, dt=torch.float32: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+    p = torch.nn.Parameter(torch.ones(200, device="cuda"))
+    plain = torch.ones(200, device="cuda")
+    loss = (p * p).sum() + (torch.ones(200, device="cuda", requires_grad=True) * plain).sum()
+    loss.backward(retain_graph=True)
+    versions = [p._version, plain._version]
+    both, grads = [p, plain], [p.grad, torch.ones(200, device="cuda")]
+    if bits == 32:
+        ops.adamw_step_multi(both, [z(200), z(200)], [z(200), z(200)], grads, [0.1] * 2, [0.0] * 2, 0.9, 0.999, 1e-8, [1, 1])
+    else:
+        ops.adamw8_step_multi(both, [z(200, dt=f8) for _ in both], [z(200, dt=f8) for _ in both], [z(2), z(2)], [z(2), z(2)], grads, [0.1] * 2, [0.0] * 2, 0.9, 0.999, 1e-8, [1, 1])
+    assert [p._version, plain._version] == [v + 1 for v in versions]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():                 # (such tensors have no counter)
+        q = torch.ones(8, device="cuda")
+        ops.adamw_step_multi([q], [z(8)], [z(8)], [torch.ones(8, device="cuda")], [0.1], [0.0], 0.9, 0.999, 1e-8, [1])
+        assert float(q[0]) < 1
+    m = splat_model(100, 16, "cuda")
+    opt = optim.FusedAdamW.for_splat_data(m, moments=bits)
+    loss = sum((t * t).sum() for t in m.params())
+    loss.backward(retain_graph=True)
+    opt.step(2000)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    if bits == 32:                               # rows of it count for the whole
+        loss = sum((t * t).sum() for t in m.params())
+        loss.backward(retain_graph=True)
+        opt.step(2001, rows=(0, 40))
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
