@@ -1303,8 +1303,8 @@ void adamw_multi(const char* op, const TensorList& params, const TensorList& exp
             if (rg == 1 && cg == (uint64_t)g.numel()) x.ld_grad = x.cols;
         }
         if (groups)
-            TORCH_CHECK(split.split > 0 && (p.numel() == 0 || (uint64_t)split.split <= x.cols), op, ": split ", split.split, " of parameter ", i,
-                        " lies beyond its ", x.cols, " columns");
+            TORCH_CHECK(split.split > 0 && (p.numel() == 0 || (uint64_t)split.split <= x.cols) && split.split <= 1ll << 31, op, ": split ", split.split,
+                        " of parameter ", i, " lies beyond its ", x.cols, " columns, or beyond 2^31 of them");
         x.param = p.data_ptr(); x.grad = g.data_ptr(); x.exp_avg = m.data_ptr(); x.exp_avg_sq = v.data_ptr();
         if (eight) {
             const int64_t runs = (p.numel() + GSX_MOMENT_RUN - 1) / GSX_MOMENT_RUN;

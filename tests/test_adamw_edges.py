@@ -139,6 +139,22 @@ def test_a_tensor_twice_is_found_wherever_it_is(count):
                     call(x)
 
 
+@pytest.mark.gpu
+def test_a_split_beyond_32_bits_is_refused():
+    """A row of 2^32 values (26 GB with its moments) has no second group at column 2^32: not one group in its place."""
+    import gsx  # noqa: F401
+    from gsx import ops
+    n = 2 ** 32 + 128
+    p = torch.empty(1, n, dtype=torch.bfloat16, device="cuda")
+    m, r = (torch.empty(1, n, dtype=torch.uint8, device="cuda").view(f8) for _ in range(2))
+    sm, sr = torch.empty(ref.runs(n), device="cuda"), torch.empty(ref.runs(n), device="cuda")
+    for split in (2 ** 32, 2 ** 32 + 64, 2 ** 31 + 1, -1, 2 ** 33):
+        with pytest.raises(RuntimeError, match="split"):
+            ops.adamw8_step_multi([p], [m], [r], [sm], [sr], [p], [0.1], [0.0], 0.9, 0.999, 1e-8, [1], splits=[(split, 0.1, 0.0, False, False)])
+    with pytest.raises(RuntimeError, match="2.31"):   # (a split within 32 bits, of rows that are too long for one)
+        ops.adamw8_step_multi([p], [m], [r], [sm], [sr], [p], [0.1], [0.0], 0.9, 0.999, 1e-8, [1], splits=[(3, 0.1, 0.0, False, False)])
+
+
 # ---- what autograd is told -------------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("bits", [32, 8])
