@@ -83,7 +83,7 @@ def step_control(device, step=0):
 
 def grad_norm_multi(grads, control, max_norm=float("inf")):
     """control[0] = the norm of all gradients (accumulated in 64 bits, the same bits every time), [1] = min(1, max_norm / (norm + 1e-6)), [2] = 1 if a gradient
-    is infinite or NaN (the updates that read the block then leave everything as it is), [3] (the step) advanced by one if none is."""
+    is infinite or NaN ([1] is 0 then, and the updates that read the block leave everything as it is), [3] (the step) advanced by one if none is."""
     _C.grad_norm_multi(grads, control, max_norm)
 
 

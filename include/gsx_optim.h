@@ -52,7 +52,7 @@ typedef struct gsx_adamw_tensor {
 
 /* Euclidean norm of all gradients, accumulated in 64 bits (the same bits every time), into the control block:
  *   [0] = norm;  [1] = min(1, max_norm / (norm + 1e-6));  [2] = 1 if any gradient is infinite or NaN, else 0;  [3] += 1 - [2].
- * max_norm: infinite for no clipping. */
+ * Where [2] is 1, [0] is infinite or NaN and [1] is 0.  max_norm: infinite for no clipping. */
 size_t gsx_grad_norm_multi_workspace_bytes(uint32_t count, const gsx_grad_tensor* tensors);
 int gsx_grad_norm_multi(uint32_t count, const gsx_grad_tensor* tensors, double max_norm, double* control, void* workspace, size_t workspace_bytes,
                         void* stream);

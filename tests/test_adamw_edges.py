@@ -155,6 +155,23 @@ def test_a_split_beyond_32_bits_is_refused():
         ops.adamw8_step_multi([p], [m], [r], [sm], [sr], [p], [0.1], [0.0], 0.9, 0.999, 1e-8, [1], splits=[(3, 0.1, 0.0, False, False)])
 
 
+# ---- the norm --------------------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_norm", [0.25, float("inf")])
+def test_the_factor_of_gradients_that_are_not_finite_is_zero(max_norm):
+    import gsx  # noqa: F401
+    from gsx import ops
+    c = ops.step_control("cuda", 3)
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        g = torch.ones(1000, device="cuda")
+        g[77] = bad
+        ops.grad_norm_multi([g], c, max_norm)
+        a = c.cpu()
+        assert not bool(torch.isfinite(a[0])) and a[1:4].tolist() == [0.0, 1.0, 3.0]
+    ops.grad_norm_multi([torch.ones(16, device="cuda")], c, max_norm)   # (the block is whole again)
+    assert c.cpu()[:4].tolist() == [4.0, min(1.0, max_norm / (4.0 + 1e-6)), 0.0, 4.0]
+
+
 # ---- what autograd is told -------------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("bits", [32, 8])
