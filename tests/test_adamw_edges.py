@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from tests import adamw_reference as ref
+from tests.test_adamw import DT, check8, check32, inputs
 
 f8 = torch.float8_e4m3fn
 
@@ -86,6 +87,156 @@ def test_codes_of_quotients_next_to_the_middle():
     want = ref.rounded(y.double(), False, u[places]) * sign
     got = m.cpu()[places].double()
     assert torch.equal(got, want.double()), "%d of %d codes" % (int((got != want).sum()), len(kept))
+
+
+# ---- many chunks, groups, views --------------------------------------------------------------------------------------------------------------------------
+def packed(x):
+    """The 8-bit state of inputs() on the device: codes and scales of both moments."""
+    (mc, ms), (rc, rs) = ref.pack(x[2], False), ref.pack(x[4], True)
+    return mc.cuda(), rc.cuda(), ms.cuda(), rs.cuda()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K,seed,hold", [(16, 3, (False, True)), (16, None, (True, False)), (25, 8, (False, False)), (9, 1, (False, True))])
+def test_adamw8_of_more_than_4096_chunks(K, seed, hold):
+    """From 4 096 chunks on a workgroup takes two: column groups followed from the first to the second, pairs that cross from one tensor into the next (odd counts of
+    chunks on every side), ends of tensors in either place of a pair."""
+    import gsx  # noqa: F401
+    from gsx import ops
+    rows = 4_300_001 // (3 * K)
+    shapes = [(1500,), (700,), (rows, K, 3), (1024,), (7, K, 3), (3 * 1024 + 5,), (2047,), (999, 4)]
+    sizes = [torch.Size(sh).numel() for sh in shapes]
+    assert sum(-(-n // 1024) for n in sizes) > 4096
+    x = inputs(sizes, torch.float32, torch.float32, K)
+    lr, wd, step = [1e-3 * (1 + i) for i in range(len(sizes))], [0.1 * (i % 3) for i in range(len(sizes))], 700
+    none = (0, 0.0, 0.0, False, False)
+    splits = [(3, 5e-4, 0.3) + hold if len(sh) == 3 else none for sh in shapes]
+    p, g = [t[0].clone().reshape(sh).cuda() for t, sh in zip(x, shapes)], [t[1].reshape(sh).cuda() for t, sh in zip(x, shapes)]
+    m, r, sm, sr = (list(c) for c in zip(*[packed(t) for t in x]))
+    ops.adamw8_step_multi(p, m, r, sm, sr, g, lr, wd, 0.9, 0.999, 1e-15, [step] * len(p), splits=splits, seed=seed)
+    for i, sh in enumerate(shapes):
+        rate, decay, held = lr[i], wd[i], None
+        if splits[i][0]:
+            second = torch.arange(sizes[i]) % (3 * K) >= 3
+            rate, decay = torch.where(second, 5e-4, lr[i]).double(), torch.where(second, 0.3, wd[i]).double()
+            held = torch.where(second, hold[1], hold[0])
+            assert torch.equal(p[i].cpu().flatten()[held], x[i][0][held])
+        check8(p[i].cpu(), m[i].cpu(), r[i].cpu(), sm[i].cpu(), sr[i].cpu(), x[i], rate, decay, step, seed=seed, ordinal=i, held=held, what=str(sh))
+
+
+def view_of(t, rows, cols, room, at):
+    """t as [rows, cols] between marked columns of a wider tensor on the device: the view, the wider tensor."""
+    wide = torch.full((rows, room), 7.0, dtype=t.dtype, device="cuda")
+    wide[:, at:at + cols] = t.reshape(rows, cols).cuda()
+    return wide[:, at:at + cols], wide
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols,split,pt,gt,seed",
+                         [shape + kind for shape in [(301, 45, 0), (301, 3, 0), (67, 45, 3), (1, 300, 7), (5, 3001, 2000)]
+                          for kind in [("f32", "f32", 4), ("f32", "f32", None), ("bf16", "bf16", 4), ("f16", "f32", 9), ("f32", "f16", 2)]] + [(95003, 45, 9, "f32", "f32", 4)])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_views_of_rows(bits, rows, cols, split, pt, gt, seed):
+    """Row-strided parameters and gradients, each alone and both (the moments are dense), with column groups, one held, and of more than 4 096 chunks: the plain form's values, and
+    the columns beside the view as they were."""
+    import gsx  # noqa: F401
+    from gsx import ops
+    n, step = rows * cols, 33
+    x = inputs([n], DT[pt], DT[gt], rows + cols)[0]
+    splits = [(split, 5e-4, 0.3, False, True)] if split else ()
+    second = torch.arange(n) % cols >= split if split else torch.zeros(n, dtype=torch.bool)
+    rate, decay = torch.where(second, 5e-4, 2e-3).double(), torch.where(second, 0.3, 0.1).double()
+    for pv, gv in ((True, True), (True, False), (False, True)):
+        p, pw = view_of(x[0], rows, cols, cols + 3, 1) if pv else (x[0].clone().reshape(rows, cols).cuda(), None)
+        g, gw = view_of(x[1], rows, cols, cols + 5, 2) if gv else (x[1].reshape(rows, cols).cuda(), None)
+        if bits == 32:
+            m, v = x[2].clone().reshape(rows, cols).cuda(), x[3].clone().reshape(rows, cols).cuda()
+            ops.adamw_step_multi([p], [m], [v], [g], [2e-3], [0.1], 0.9, 0.999, 1e-15, [step], splits=splits)
+            live = ~second
+            check32(p.cpu().flatten()[live], m.cpu().flatten()[live], v.cpu().flatten()[live], [t[live] for t in x], rate[live], decay[live], step)
+            assert torch.equal(m.cpu().flatten()[second], x[2][second]) and torch.equal(v.cpu().flatten()[second], x[3][second])
+        else:
+            m, r, sm, sr = packed(x)
+            ops.adamw8_step_multi([p], [m], [r], [sm], [sr], [g], [2e-3], [0.1], 0.9, 0.999, 1e-15, [step], splits=splits, seed=seed)
+            check8(p.cpu(), m.cpu(), r.cpu(), sm.cpu(), sr.cpu(), x, rate, decay, step, seed=seed, held=second)
+        assert torch.equal(p.cpu().flatten()[second], x[0][second]) and torch.equal(g.cpu().flatten(), x[1])
+        for w, at in ((pw, 1), (gw, 2)):
+            assert w is None or (bool((w[:, :at] == 7).all()) and bool((w[:, at + cols:] == 7).all()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols,split", [(3, 70001, 65537), (2, 65536, 65535), (40, 70001, 1), (2, 1 << 21, 1 << 20)])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_column_groups_of_long_rows(bits, rows, cols, split):
+    """Rows of more than 65 535 values, whose columns are found by another quotient."""
+    import gsx  # noqa: F401
+    from gsx import ops
+    n = rows * cols
+    x = inputs([n], torch.float32, torch.float32, cols % 1000)[0]
+    second = torch.arange(n) % cols >= split
+    rate, decay = torch.where(second, 5e-4, 2e-3).double(), torch.where(second, 0.3, 0.1).double()
+    p, g = x[0].clone().reshape(rows, cols).cuda(), x[1].reshape(rows, cols).cuda()
+    splits = [(split, 5e-4, 0.3, False, False)]
+    if bits == 32:
+        m, v = x[2].clone().cuda(), x[3].clone().cuda()
+        ops.adamw_step_multi([p], [m], [v], [g], [2e-3], [0.1], 0.9, 0.999, 1e-15, [50], splits=splits)
+        check32(p.cpu().flatten(), m.cpu(), v.cpu(), x, rate, decay, 50)
+    else:
+        m, r, sm, sr = packed(x)
+        ops.adamw8_step_multi([p], [m], [r], [sm], [sr], [g], [2e-3], [0.1], 0.9, 0.999, 1e-15, [50], splits=splits, seed=2)
+        check8(p.cpu(), m.cpu(), r.cpu(), sm.cpu(), sr.cpu(), x, rate, decay, 50, seed=2)
+
+
+@pytest.mark.gpu
+def test_adamw_of_more_than_two_to_the_23_chunks():
+    """Beyond 2^23 chunks (2^33 values, 103 GB here) a workgroup of the 32-bit update takes two of them as well; two column groups in rows of 48."""
+    import gsx  # noqa: F401
+    from gsx import ops
+    rows = 2 ** 33 // 48 + 1000
+    assert -(-rows * 48 // 1024) > 2 ** 23
+    p, g = (torch.zeros(rows, 48, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    m, v = (torch.zeros(rows, 48, device="cuda") for _ in range(2))
+    spots = [0, rows // 3, 2 ** 32 // 48 - 30, rows - 60]
+    x = inputs([60 * 48 * len(spots)], torch.bfloat16, torch.bfloat16, 3)[0]
+    parts = [[t[60 * 48 * i:60 * 48 * (i + 1)] for t in x] for i in range(len(spots))]
+    for at, part in zip(spots, parts):
+        for dst, src in ((p, part[0]), (g, part[1]), (m, part[2]), (v, part[3])):
+            dst[at:at + 60] = src.reshape(60, 48).cuda()
+    ops.adamw_step_multi([p], [m], [v], [g], [2e-3], [0.1], 0.9, 0.999, 1e-8, [50], splits=[(3, 5e-4, 0.3, False, False)])
+    second = torch.arange(60 * 48) % 48 >= 3
+    rate, decay = torch.where(second, 5e-4, 2e-3).double(), torch.where(second, 0.3, 0.1).double()
+    for at, part in zip(spots, parts):
+        check32(*[t[at:at + 60].cpu().flatten() for t in (p, m, v)], part, rate, decay, 50, eps=1e-8)
+    for a, b in zip(spots, spots[1:]):      # between the places: zeros stay zeros
+        at = (a + b) // 2
+        assert float(p[at:at + 100].abs().max()) == 0 and float(m[at:at + 100].abs().max()) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gt", ["f32", "bf16", "mixed"])
+def test_norm_of_more_than_2048_chunks(gt):
+    """Chunks of 4 096 values; beyond 2 048 of them a workgroup takes several, here of one tensor, across ends of tensors, and of views."""
+    import gsx  # noqa: F401
+    from gsx import ops
+    kinds = [torch.float32, torch.bfloat16, torch.float16]
+    sizes = [9_000_003, 5, 4097, 8191, 1, 0, 12_289, 4096, 7_000_001]
+    gs = [inputs([n], torch.float32, DT[gt] if gt != "mixed" else kinds[i % 3], 60 + i)[0][1] for i, n in enumerate(sizes)]
+    want = sum(float((g.double() ** 2).sum()) for g in gs)
+    dev = [g.cuda() for g in gs]
+    rows = 4_400_000 // 45
+    sh = torch.randn(rows, 16, 3, generator=torch.Generator().manual_seed(1)).to(gs[0].dtype)
+    dev.append(sh.cuda()[:, 1:])
+    want = (want + float((sh[:, 1:].double() ** 2).sum())) ** 0.5
+    c = ops.step_control("cuda")
+    bits = []
+    for _ in range(3):
+        ops.grad_norm_multi(dev, c)
+        bits.append(c.cpu()[0])
+    # 64-bit sums of at most 2^25 squares in any order: 2^25 * 2^-53 of the sum at most, half of it on the root, the same again for the sums here
+    assert abs(float(bits[0]) - want) <= 2.0 ** -27 * want and bits[0] == bits[1] == bits[2] and c[3] == 3 and c[4] == 0
+    views = [sh.cuda()[:, :1], sh.cuda()[:, 1:]]
+    ops.grad_norm_multi(views, c)
+    assert abs(float(c[0]) / float(sh.double().norm()) - 1) < 2.0 ** -27
 
 
 # ---- what is refused -----------------------------------------------------------------------------------------------------------------------------------
