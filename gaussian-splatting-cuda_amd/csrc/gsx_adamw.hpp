@@ -140,8 +140,8 @@ struct Betas {
     uint32_t seed;
 };
 
-// 1 - exp(x), x <= 0, to a few 2^-24 of itself: the series where it is small, where 1 - exp(x) would lose its leading digits (beta2 = 0.999, first step: 1e-4 of it).
-// A third of the library's expm1f in instructions; every workgroup computes it.
+// 1 - exp(x), x <= 0, to 6 * 2^-24 of itself (x is rounded too): the series where it is small, where 1 - exp(x) would lose its leading digits (beta2 = 0.999, first step: 1e-4
+// of it).  A third of the library's expm1f in instructions; every workgroup computes it.
 GSX_DEV float one_minus_exp(float x) {
     float s = 1.0f / 40320.0f;   // (1 + x/2 + x^2/6 + ...: what is cut is below x^8 / 9!, 2^-26 at -1/2)
     s = fmaf(s, x, 1.0f / 5040.0f); s = fmaf(s, x, 1.0f / 720.0f); s = fmaf(s, x, 1.0f / 120.0f);

@@ -59,7 +59,9 @@ int gsx_grad_norm_multi(uint32_t count, const gsx_grad_tensor* tensors, double m
 
 /* AdamW with decoupled decay, t the step, g the gradient (times the control block's factor where there is one):
  *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;  p = p (1 - lr wd) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
- * in 32 bits, p rounded once to its type; an eps below 2^-126 (0 too) counts as 2^-126.  control: NULL, or a control block; needed where a step is 0. */
+ * in 32 bits, p rounded once to its type; an eps below 2^-126 (0 too) counts as 2^-126.  control: NULL, or a control block; needed where a step is 0.
+ * 1 / (1 - beta1^t) and 1 / sqrt(1 - beta2^t) of a step of the list are formed in 64 bits and rounded; those of the control block's step on the device, in 32 bits, to within
+ * 2^-21 of themselves.  The quotient by the root is a product with a reciprocal of 1 unit in the last place. */
 int gsx_adamw_step_multi(uint32_t count, const gsx_adamw_tensor* tensors, double beta1, double beta2, double eps, const double* control, void* stream);
 
 /* The same with m and r = sqrt(v) stored as OCP e4m3 numbers, one scale for each GSX_MOMENT_RUN consecutive values (the last run of a tensor may be

@@ -1,5 +1,8 @@
 """The optimizer operators over many tensors (include/gsx_optim.h) at their edges: quotients next to the middle between two numbers, runs of chunks that cross from tensor
 to tensor, views with 8-bit moments, what is refused, what autograd is told — against the plain forms in 64 bits (adamw_reference.py)."""
+import os
+import socket
+
 import pytest
 import torch
 
@@ -362,3 +365,153 @@ def test_a_backward_over_a_step_is_refused(bits):
         opt.step(2001, rows=(0, 40))
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             loss.backward()
+
+
+# ---- what comes of many steps ----------------------------------------------------------------------------------------------------------------------------
+def test_the_plain_form_rounded_to_nearest_comes_to_rest():
+    """The walk that the next test's moments take, by the definition alone: 1.75, 2.5, 3, ... 6.5 codes, where 6.5 sqrt(0.999 + 0.001 (56 / 6.5)^2) = 6.73 rounds back."""
+    code, walk = 0.0, []
+    for _ in range(20):
+        code = float(ref.rounded(torch.tensor([(0.999 * code ** 2 + 0.001 * 56.0 ** 2) ** 0.5], dtype=torch.float64), True, None))
+        walk.append(code)
+    assert walk[:10] == [1.75, 2.5, 3.0, 3.5, 4.0, 4.5, 5.0, 5.5, 6.0, 6.5] and set(walk[10:]) == {6.5}
+
+
+@pytest.mark.gpu
+def test_moments_rounded_to_nearest_come_to_rest():
+    """A constant gradient, 1 / 8 of the one that holds the run's scale (whose moment is at its end from the start): to nearest, the second moment stops after ten steps at
+    (6.5 / 56)^2 = 1.3 % of where it belongs and stays; stochastically it goes on."""
+    import gsx  # noqa: F401
+    from gsx import ops
+    n = 128 * 16
+    last = {}
+    for seed in (None, 11):
+        p, g = torch.zeros(n, device="cuda"), torch.full((n,), 1e-3, device="cuda")
+        g[::128] = 8e-3
+        m, r = (torch.zeros(n, dtype=torch.uint8, device="cuda").view(f8) for _ in range(2))
+        sm, sr = torch.zeros(n // 128, device="cuda"), torch.full((n // 128,), 8e-3 / 448, device="cuda")
+        r.view(torch.uint8)[::128] = 0x7E        # 448
+        keep = torch.arange(n, device="cuda") % 128 != 0
+        for t in range(1, 401):
+            ops.adamw8_step_multi([p], [m], [r], [sm], [sr], [g], [0.0], [0.0], 0.9, 0.999, 1e-8, [t], seed=seed)
+            if seed is None and t in (9, 10, 100, 400):
+                assert bool((r.float()[keep] == (6.0 if t == 9 else 6.5)).all()), t
+        last[seed] = float(((r.float() * sr.repeat_interleave(128))[keep] ** 2).mean()) / 1e-6
+    # stochastically: 1 - 0.999^400 = 0.33 of it, the mean within the walk's 0.25 / sqrt(n) a standard error (five of them) and 3 %
+    assert last[None] < 0.0136 and abs(last[11] / (1 - 0.999 ** 400) - 1) < 0.03 + 5 * 0.25 / n ** 0.5, last
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("optimizer", ["adamw", "adamw8"])
+def test_the_same_training_twice(optimizer):
+    """Growth, relocation and reordering on the way: the same rows, steps and moments' sizes both times."""
+    import gsx  # noqa: F401
+    from gsx import rasterizer, strategy, trainer
+    from tests.test_gpu_training import _scene
+    seen = []
+    for _ in range(2):
+        sc, model, cams = _scene("cuda:0")
+        bg = sc["background"].to("cuda:0")
+        with torch.no_grad():
+            images = [rasterizer.rasterize_fused(c, model, bg).image.clone() for c in cams]
+        model.means = (model.means + 0.01 * torch.randn(model.means.shape, generator=torch.Generator().manual_seed(1)).cuda()).contiguous()
+        params = strategy.OptimizationParameters(iterations=45, start_refine=10, refine_every=15, stop_refine=40, max_cap=3200)
+        tr = trainer.Trainer(model, cams, images, params, bg, seed=1, optimizer=optimizer, optimizer_options={"max_grad_norm": 0.05})
+        tr.train(45)
+        opt = tr.strategy.optimizer
+        seen.append((model.means.shape[0], opt.steps, float(opt.control[3]), {k: {n: tuple(t.shape) for n, t in st.items()} for k, st in opt.state.items()}))
+    assert seen[0] == seen[1]
+
+
+@pytest.mark.gpu
+def test_bias_corrections_of_the_device_and_of_the_call():
+    """A step counted on the device forms its corrections in 32 bits, one of the call in 64: 1 / (1 - beta1^t) within 8 * 2^-24 (the series or the exponential 6, the
+    reciprocal 2), 1 / sqrt(1 - beta2^t) within 5; from p = 0 the two updates differ by those, half a unit each of the other, and seven roundings on either side."""
+    import gsx  # noqa: F401
+    from gsx import ops
+    x = inputs([1000], torch.float32, torch.float32, 14)[0]
+    for betas in ((0.9, 0.999), (0.5, 0.9), (0.99, 0.99999), (0.0, 0.0)):
+        for t in (1, 2, 3, 6, 7, 8, 50, 400, 499, 500, 501, 690, 700, 1000, 5000, 30000, 10 ** 6, 2 ** 32 - 1):
+            out = []
+            for steps, c in (([t], None), ([], ops.step_control("cuda", t))):
+                p, m, v = torch.zeros(1000, device="cuda"), x[2].clone().cuda(), x[3].clone().cuda()
+                ops.adamw_step_multi([p], [m], [v], [x[1].cuda()], [1e-2], [0.0], *betas, 1e-8, steps, control=c)
+                out.append(p.cpu().double())
+            a, b = out
+            assert bool(((a - b).abs() <= 28 * ref.U * a.abs() + 2.0 ** -148).all()), (betas, t, float(((a - b).abs() / a.abs().clamp(min=1e-300)).max() / ref.U))
+
+
+# ---- over ranks --------------------------------------------------------------------------------------------------------------------------------------------
+def _plain_adamw(params, exp_avgs, exp_avg_sqs, grads, lrs, weight_decays, beta1, beta2, eps, steps, control=None, splits=()):
+    """ops.adamw_step_multi in torch operations of float32 on the CPU, value by value (so that a block of rows has the bits of the whole)."""
+    assert control is None and len(splits) == len(params)
+    for p, m, v, g, lr, wd, t, (split, lr_b, wd_b, hold_a, hold_b) in zip(params, exp_avgs, exp_avg_sqs, grads, lrs, weight_decays, steps, splits):
+        cols = p.numel() // max(1, p.shape[0])
+        second = ((torch.arange(cols) >= split) if split else torch.zeros(cols, dtype=torch.bool)).reshape(p.shape[1:])
+        rate, decay = torch.where(second, lr_b, lr), torch.where(second, wd_b, wd)
+        live = ~torch.where(second, torch.tensor(bool(hold_b)), torch.tensor(bool(hold_a)))
+        m1, v1 = beta1 * m + (1 - beta1) * g, beta2 * v + (1 - beta2) * g * g
+        p1 = p - rate * decay * p - rate / (1 - beta1 ** t) * m1 / (v1.sqrt() / (1 - beta2 ** t) ** 0.5 + eps)
+        for old, new in ((m, m1), (v, v1), (p, p1)):
+            old.copy_(torch.where(live, new, old))
+
+
+def _sharded_adamw_worker(rank, world, port, out):
+    os.environ.update(RANK=str(rank), LOCAL_RANK=str(rank), WORLD_SIZE=str(world), MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    import torch.distributed as dist
+
+    import gsx  # noqa: F401
+    from gsx import distributed as gdist
+    from gsx import ops, optim
+    from tests.test_adamw import splat_model
+    ops.adamw_step_multi = _plain_adamw          # (the kernel needs a GPU)
+    gdist.init_from_env(backend="gloo")
+    models = {mode: splat_model(101, 16, "cpu", seed=4) for mode in ("whole", "rows")}
+    opts = {mode: optim.FusedAdamW.for_splat_data(m, weight_decay={"shN": 0.2, "opacity": 0.1}) for mode, m in models.items()}
+    sharded = gdist.ShardedAdam(opts["rows"])
+    buckets = {mode: gdist.GradBucket(m.params()) for mode, m in models.items()}
+    for t in range(8):
+        if t in (3, 6):                          # growth by 5 rows, then (6) a permutation and a removal behind it
+            for mode, m in models.items():
+                for name in ("means", "sh", "scaling_raw", "rotation_raw", "opacity_raw"):
+                    old = getattr(m, name).detach()
+                    setattr(m, name, torch.cat([old, 0.5 * old[:5]]).requires_grad_(True))
+                opts[mode].extend_state(5)
+        if t == 6:
+            sharded.merge_moments()
+            order = torch.randperm(models["rows"].means.shape[0], generator=torch.Generator().manual_seed(3))[:-2]
+            for mode, m in models.items():
+                for name in ("means", "sh", "scaling_raw", "rotation_raw", "opacity_raw"):
+                    setattr(m, name, getattr(m, name).detach()[order].clone().requires_grad_(True))
+                opts[mode].select_state(order)
+        if t in (3, 6):
+            buckets = {mode: gdist.GradBucket(m.params()) for mode, m in models.items()}
+        gen = torch.Generator().manual_seed(100 * t + rank)   # this rank's camera
+        for a, b in zip(models["whole"].params(), models["rows"].params()):
+            a.grad.copy_(torch.randn(a.shape, generator=gen))
+            b.grad.copy_(a.grad)
+        buckets["whole"].all_reduce_mean()
+        opts["whole"].step(997 + t)              # shN held for the first four
+        sharded.step(997 + t, buckets["rows"])
+        for a, b in zip(models["whole"].params(), models["rows"].params()):
+            assert torch.equal(a, b), (rank, t)
+    sharded.merge_moments()
+    for key, st in opts["whole"].state.items():
+        for name in ("exp_avg", "exp_avg_sq"):
+            assert torch.equal(st[name], opts["rows"].state[key][name]), (rank, key, name)
+    assert float(opts["rows"].state["sh"]["exp_avg"][:, 1:].abs().max()) > 0 and opts["rows"].steps == 8
+    with pytest.raises(RuntimeError, match="row sharding"):
+        gdist.ShardedAdam(optim.FusedAdamW.for_splat_data(models["rows"], moments=8), buckets["rows"]).step(2000)
+    torch.save([p.detach() for p in models["rows"].params()], os.path.join(out, "rank%d.pt" % rank))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_sharded_adamw_over_two_ranks(tmp_path):
+    """distributed.ShardedAdam with FusedAdamW on two ranks, through growth, reordering and removal: the bits of the whole step on every rank, parameters and moments."""
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    torch.multiprocessing.spawn(_sharded_adamw_worker, args=(2, port, str(tmp_path)), nprocs=2, join=True)
+    a, b = (torch.load(str(tmp_path / ("rank%d.pt" % r)), weights_only=True) for r in range(2))
+    assert all(torch.equal(x, y) for x, y in zip(a, b)) and a[0].shape == (109, 3)
