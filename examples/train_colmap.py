@@ -4,7 +4,7 @@ eval/default_optimization_params.json`), on this backend:
 
     python examples/train_colmap.py -d data/garden --images images_4 --iter 30000 [--config params.json] [--eval] [--test-every 8]
                                     [-o out_dir] [--json out.json] [--max-width 3840] [--resize-factor -1]
-                                    [--optimizer adam | adamw | adamw8] [--max-grad-norm 0]
+                                    [--optimizer adam | adamw | adamw8] [--weight-decay 0] [--max-grad-norm 0]
 
     COLMAP sparse model (io_colmap.load_colmap: cameras / images / points3D .bin or .txt, `images_<k>` scales the intrinsics as upstream)
     -> images decoded and resized as Camera::load_and_get_image does (io_image) -> SplatData::init_model_from_pointcloud
@@ -108,8 +108,13 @@ def run(args):
     model, scene_scale = io_colmap.init_model_from_pointcloud(scene.points, scene.colors, scene.scene_center, sh_degree=params.sh_degree,
                                                              init_scaling=params.init_scaling, init_opacity=params.init_opacity, device=dev)
     bg = torch.zeros(3, device=dev)
+    options = {}
+    if getattr(args, "weight_decay", 0.0):
+        options["weight_decay"] = {"shN": args.weight_decay}
+    if getattr(args, "max_grad_norm", 0.0):
+        options["max_grad_norm"] = args.max_grad_norm
     tr = trainer.Trainer(model, [cams[i] for i in train_idx], [images[i] for i in train_idx], params, bg, scene_scale=scene_scale, seed=0, optimizer=getattr(args, "optimizer", "adam"),
-                         optimizer_options={"max_grad_norm": args.max_grad_norm} if getattr(args, "max_grad_norm", 0.0) else None)
+                         optimizer_options=options or None)
     t_load = time.perf_counter() - t_load
     ev_idx = test_idx if test_idx else train_idx[::8]
     ev = lambda: metrics.evaluate(model, [cams[i] for i in ev_idx], [images[i] for i in ev_idx], bg)  # noqa: E731
@@ -151,6 +156,7 @@ def main():
     ap.add_argument("--resize-factor", type=int, default=-1)
     ap.add_argument("--max-width", type=int, default=3840)
     ap.add_argument("--optimizer", choices=("adam", "adamw", "adamw8"), default="adam", help="adamw8: AdamW with both moments in 8 bits")
+    ap.add_argument("--weight-decay", type=float, default=0.0, help="adamw / adamw8: decoupled decay of the view-dependent colour (the shN group)")
     ap.add_argument("--max-grad-norm", type=float, default=0.0, help="adamw / adamw8: clip the gradients to this norm (0: no clip)")
     ap.add_argument("-o", "--output", default=None, help="directory for the trained model's PLY")
     ap.add_argument("--json", default=None)

@@ -6,7 +6,7 @@ start_refine 500, refine_every 100, max_cap 1M), strategy forced to MCMC (the on
 SURVEY §8f-3).  Ground-truth images are renders of a hidden 400 k-Gaussian scene; the trainee starts from 200 k of its points
 (positions jittered, as an SfM cloud would be) through init_model_from_pointcloud and grows to the 1 M cap.
 
-    python examples/train_garden_standin.py [iterations=4000] [--json out.json] [--profile-ops] [--optimizer=adam | adamw | adamw8]
+    python examples/train_garden_standin.py [iterations=4000] [--json out.json] [--profile-ops] [--optimizer=adam | adamw | adamw8] [--weight-decay=0]
 
 Prints one JSON line: iterations/s (whole loop, incl. densification), PSNR before / after over 24 held-in cameras, Gaussian count.
 """
@@ -89,7 +89,8 @@ def main():
     iters = int(args[0]) if args else 4000
     out_json = sys.argv[sys.argv.index("--json") + 1] if "--json" in sys.argv else None
     optimizer = next((a.split("=", 1)[1] for a in sys.argv[1:] if a.startswith("--optimizer=")), "adam")
-    tr, model, cams, images, bg, params = setup(optimizer=optimizer)
+    decay = next((float(a.split("=", 1)[1]) for a in sys.argv[1:] if a.startswith("--weight-decay=")), 0.0)   # of the view-dependent colour
+    tr, model, cams, images, bg, params = setup(optimizer=optimizer, optimizer_options={"weight_decay": {"shN": decay}} if decay else None)
     eval_idx = list(range(0, N_CAMS, 8))
     ev = lambda: metrics.evaluate(model, [cams[i] for i in eval_idx], [images[i] for i in eval_idx], bg)  # noqa: E731
     before = ev()
@@ -111,7 +112,7 @@ def main():
     t34, _ = marks[3 * iters // 4]
     res = {"workload": "garden stand-in (BASELINE configs[2]): %d ring cameras @%dx%d, hidden scene of %d Gaussians, init %d, MCMC to max_cap %d, "
                        "parameter preset 'default' (default_optimization_params.json)" % (N_CAMS, W, H, N_GT, N_INIT, params.max_cap),
-           "optimizer": optimizer, "iterations": iters, "seconds": round(dt, 2), "iters_per_s": round(iters / dt, 1),
+           "optimizer": optimizer, "weight_decay": decay, "iterations": iters, "seconds": round(dt, 2), "iters_per_s": round(iters / dt, 1),
            "iters_per_s_last_quarter": round((iters - 3 * iters // 4) / (dt - t34), 1),
            "gaussians_start": N_INIT, "gaussians_end": int(model.means.shape[0]),
            "gaussians_at": {str(k): v[1] for k, v in marks.items()},

@@ -1,7 +1,7 @@
 """End-to-end example on a GPU box: fit a perturbed Gaussian cloud to renders of the original with the `--gut` training step
 (MCMC strategy, fused L1 + SSIM loss, fused Adam), report PSNR / SSIM, export and re-import the model as a 3DGS PLY.
 
-    python examples/train_synthetic.py [iterations] [adam | adamw | adamw8]
+    python examples/train_synthetic.py [iterations] [adam | adamw | adamw8] [decay of the view-dependent colour]
 """
 import math
 import os
@@ -18,6 +18,7 @@ from gsx import io_ply, metrics, rasterizer, scenes, strategy, trainer  # noqa: 
 def main():
     iters = int(sys.argv[1]) if len(sys.argv) > 1 else 400
     optimizer = sys.argv[2] if len(sys.argv) > 2 else "adam"
+    options = {"weight_decay": {"shN": float(sys.argv[3])}} if len(sys.argv) > 3 else None
     dev = "cuda:0"
     sc = scenes.scene_small(seed=5, N=20000)
     gt = scenes.to_splat_data(sc, dev)
@@ -37,7 +38,7 @@ def main():
     model.means = (gt.means + 0.01 * torch.randn(gt.means.shape, generator=g).to(dev)).contiguous()
     params = strategy.OptimizationParameters(iterations=iters, start_refine=iters // 8, refine_every=max(1, iters // 8), stop_refine=iters,
                                              max_cap=22000)
-    tr = trainer.Trainer(model, cams, images, params, bg, seed=0, optimizer=optimizer)
+    tr = trainer.Trainer(model, cams, images, params, bg, seed=0, optimizer=optimizer, optimizer_options=options)
 
     def evaluate():
         r = metrics.evaluate(model, cams, images, bg)

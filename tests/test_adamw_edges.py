@@ -1,7 +1,11 @@
 """The optimizer operators over many tensors (include/gsx_optim.h) at their edges: quotients next to the middle between two numbers, runs of chunks that cross from tensor
 to tensor, views with 8-bit moments, what is refused, what autograd is told — against the plain forms in 64 bits (adamw_reference.py)."""
+import argparse
+import importlib.util
 import os
 import socket
+import sys
+import types
 
 import pytest
 import torch
@@ -515,3 +519,69 @@ def test_sharded_adamw_over_two_ranks(tmp_path):
     torch.multiprocessing.spawn(_sharded_adamw_worker, args=(2, port, str(tmp_path)), nprocs=2, join=True)
     a, b = (torch.load(str(tmp_path / ("rank%d.pt" % r)), weights_only=True) for r in range(2))
     assert all(torch.equal(x, y) for x, y in zip(a, b)) and a[0].shape == (109, 3)
+
+
+# ---- the training examples -----------------------------------------------------------------------------------------------------------------------------------
+def _example(name):
+    spec = importlib.util.spec_from_file_location(name, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", name + ".py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
+@pytest.mark.parametrize("name", ["train_colmap", "train_synthetic", "train_garden_standin"])
+def test_examples_hand_their_decay_to_the_optimizer(name, monkeypatch):
+    """The command's decay arrives as the Trainer's option, up to which a stand-in takes the place of what needs a GPU."""
+    mod = _example(name)
+    seen = {}
+    argv = {"train_colmap": ["-d", "x", "--optimizer", "adamw8", "--weight-decay", "0.25", "--max-grad-norm", "2"], "train_synthetic": ["10", "adamw8", "0.25"],
+            "train_garden_standin": ["10", "--optimizer=adamw8", "--weight-decay=0.25"]}[name]
+    monkeypatch.setattr(sys, "argv", [name] + argv)
+
+    class Reached(Exception):
+        pass
+
+    def stop(*args, **kw):
+        seen.update(kw)
+        raise Reached
+    if name == "train_garden_standin":
+        monkeypatch.setattr(mod, "setup", stop)
+    elif name == "train_colmap":
+        scene = types.SimpleNamespace(points=[0], colors=None, scene_center=None, cameras=[], load_images=lambda *a, **kw: [])
+        monkeypatch.setattr(mod.io_colmap, "load_colmap", lambda *a, **kw: scene)
+        monkeypatch.setattr(mod.io_colmap, "init_model_from_pointcloud", lambda *a, **kw: (None, 1.0))
+        monkeypatch.setattr(mod.trainer, "Trainer", stop)
+    else:
+        monkeypatch.setattr(mod.trainer, "Trainer", stop)
+        monkeypatch.setattr(mod.rasterizer, "rasterize_fused", lambda *a, **kw: types.SimpleNamespace(image=torch.zeros(3, 4, 4)))
+    on_cpu = lambda f: lambda *a, **kw: f(*[("cpu" if isinstance(x, str) and x.startswith("cuda") else x) for x in a], **{k: "cpu" if k == "device" else v for k, v in kw.items()})  # noqa: E731
+    monkeypatch.setattr(torch, "zeros", on_cpu(torch.zeros))
+    monkeypatch.setattr(torch.Tensor, "to", on_cpu(torch.Tensor.to))
+    with pytest.raises(Reached):
+        mod.main()
+    assert seen["optimizer"] == "adamw8" and seen["optimizer_options"]["weight_decay"] == {"shN": 0.25}
+    assert seen["optimizer_options"].get("max_grad_norm", 2.0) == 2.0 and (name != "train_colmap" or "max_grad_norm" in seen["optimizer_options"])
+
+
+@pytest.mark.gpu
+def test_train_colmap_example_with_decay(tmp_path):
+    """The command, for a few iterations, without and with a decay: it reaches its group and no other."""
+    mod = _example("train_colmap")
+    cap = mod.make_synthetic(str(tmp_path / "capture"))
+    kept, make = [], mod.trainer.Trainer
+
+    def keep(*a, **kw):
+        kept.append(make(*a, **kw))
+        return kept[-1]
+    for decay in (0.0, 0.5):
+        args = argparse.Namespace(data=cap, images="images", iter=25, config=None, eval=True, test_every=8, resize_factor=-1, max_width=3840, output=None, json=None, log_every=0,
+                                  optimizer="adamw", weight_decay=decay, max_grad_norm=1.0)
+        mod.trainer.Trainer = keep
+        try:
+            res = mod.run(args)
+        finally:
+            mod.trainer.Trainer = make
+        assert res["iterations"] == 25
+    a, b = (t.strategy.optimizer for t in kept)
+    assert a.weight_decay["shN"] == 0.0 and b.weight_decay == dict(a.weight_decay, shN=0.5) and b.max_grad_norm == 1.0
+    assert a.steps == b.steps == 24              # (the last iteration of a run takes no step: MCMC.step)
