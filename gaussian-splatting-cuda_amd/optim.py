@@ -208,7 +208,10 @@ class FusedAdamW(FusedAdam):
                    device, nothing waits.  float("inf"): the check alone.  last_norm() and skipped_last() read the outcome (they wait).
 
     All groups share one step count; with max_grad_norm it is on the device and counts the steps that were not skipped.  The shN group is held during the first
-    1000 iterations like FusedAdam's (its moments stay zero).  The SH step is not fused into the render backward (begin_fused_sh_step returns None)."""
+    1000 iterations like FusedAdam's (its moments stay zero).  The SH step is not fused into the render backward (begin_fused_sh_step returns None).
+
+    A step can be captured into a graph once a step has made the moments, with max_grad_norm (float("inf") will do), which counts the replays on the device; rates and
+    the hold are the captured step's."""
 
     def __init__(self, model, lrs, betas=(0.9, 0.999), eps=1e-15, skip_sh_steps=False, weight_decay=None, moments=32, max_grad_norm=None, seed=0):
         if moments not in (32, 8):
@@ -313,6 +316,11 @@ class FusedAdamW(FusedAdam):
         names = [n for n in GROUPS if n != "shN" and self._param(n).grad is not None]
         if not names:
             return
+        if self._param(names[0]).is_cuda and torch.cuda.is_current_stream_capturing():
+            if self.max_grad_norm is None:
+                raise RuntimeError("FusedAdamW: a captured step without max_grad_norm would repeat its step number in every replay (float(\"inf\") counts on the device)")
+            if self.control is None or any(_ATTR[n] not in self.state for n in names):
+                raise RuntimeError("FusedAdamW: the first step makes the moments and the step count, which every replay would make anew: take one before the capture")
         self.steps += 1
         params = [self._param(n) for n in names]
         grads = [r(p.grad) for p in params]

@@ -445,6 +445,51 @@ def test_bias_corrections_of_the_device_and_of_the_call():
             assert bool(((a - b).abs() <= 28 * ref.U * a.abs() + 2.0 ** -148).all()), (betas, t, float(((a - b).abs() / a.abs().clamp(min=1e-300)).max() / ref.U))
 
 
+# ---- captured steps of a model ---------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("moments", [32, 8])
+def test_captured_steps_of_a_model(moments):
+    """FusedAdamW.step in a graph: replays equal eager steps, the step counted on the device, with eager work between them.  What would come out wrong in every replay is
+    refused: the step that makes the moments, and a step number that is the call's."""
+    import gsx  # noqa: F401
+    from gsx import optim
+    from tests.test_adamw import splat_model
+    models = [splat_model(211, 16, "cuda") for _ in range(2)]
+    opts = [optim.FusedAdamW.for_splat_data(m, moments=moments, max_grad_norm=0.5, weight_decay={"shN": 0.1}) for m in models]
+    uncounted = optim.FusedAdamW.for_splat_data(splat_model(211, 16, "cuda"), moments=moments)
+    fresh = optim.FusedAdamW.for_splat_data(splat_model(211, 16, "cuda"), moments=moments, max_grad_norm=float("inf"))
+
+    def gradients(t):
+        for m in models + [uncounted.model, fresh.model]:
+            for i, p in enumerate(m.params()):
+                g = torch.randn(p.shape, generator=torch.Generator().manual_seed(10 * t + i)).cuda()
+                p.grad = g if p.grad is None else p.grad.copy_(g)
+    gradients(0)
+    for o in opts + [uncounted]:
+        o.step(2000)
+    torch.cuda.synchronize()
+    graph, x = torch.cuda.CUDAGraph(), torch.zeros(8, device="cuda")
+    with torch.cuda.graph(graph):
+        x.add_(1)
+        for o, match in ((uncounted, "max_grad_norm"), (fresh, "before the capture")):
+            with pytest.raises(RuntimeError, match=match):
+                o.step(2001)
+        opts[1].step(2001)
+    assert uncounted.steps == 1 and fresh.steps == 0 and not fresh.state and fresh.control is None
+    for t in range(1, 5):
+        gradients(t)
+        opts[0].step(2001)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(models[0].params(), models[1].params()):
+            assert torch.equal(a, b), t
+        for k, st in opts[0].state.items():
+            assert all(torch.equal(v.view(torch.uint8), opts[1].state[k][n].view(torch.uint8)) for n, v in st.items())
+        assert torch.equal(opts[0].control, opts[1].control) and float(opts[1].control[3]) == t + 1
+    fresh.step(2001)
+    assert fresh.steps == 1 and float(x[0]) == 4
+
+
 # ---- over ranks --------------------------------------------------------------------------------------------------------------------------------------------
 def _plain_adamw(params, exp_avgs, exp_avg_sqs, grads, lrs, weight_decays, beta1, beta2, eps, steps, control=None, splits=()):
     """ops.adamw_step_multi in torch operations of float32 on the CPU, value by value (so that a block of rows has the bits of the whole)."""
