@@ -100,7 +100,8 @@ def adamw_step_multi(params, exp_avgs, exp_avg_sqs, grads, lrs, weight_decays, b
 def adamw8_step_multi(params, exp_avgs, exp_rmss, avg_scales, rms_scales, grads, lrs, weight_decays, beta1, beta2, eps, steps, control=None, splits=(), seed=None):
     """adamw_step_multi with the first moment and the root of the second as float8_e4m3fn tensors, each with one float32 scale for MOMENT_RUN consecutive values
     (float32 [ceil(numel / MOMENT_RUN)]; zeros are zero moments).  seed None: rounded to nearest; 0 .. 2^32 - 1: stochastically, another draw for
-    every step, tensor of the list and value.  With rounding to nearest a moment that changes by less than half a step of the format (3 to 6 %) does not
+    every step, tensor of the list and value.  A held group's parameters stay as they are, its moments as values: they are rounded anew with their run, whose scale the
+    other group may move.  With rounding to nearest a moment that changes by less than half a step of the format (3 to 6 %) does not
     change at all, and the second moment's average over 1 / (1 - beta2) steps comes to rest: training takes a seed."""
     _C.adamw8_step_multi(params, exp_avgs, exp_rmss, avg_scales, rms_scales, grads, lrs, weight_decays, beta1, beta2, eps, steps, control, splits, seed)
 

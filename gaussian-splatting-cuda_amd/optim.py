@@ -293,7 +293,7 @@ class FusedAdamW(FusedAdam):
         sts = list(self.state.values())
         if sts:
             names = ("exp_avg", "exp_rms", "avg_scale", "rms_scale")
-            new = ops.adamw8_select_rows(*[[st[k] for st in sts] for k in names], indices.contiguous())
+            new = ops.adamw8_select_rows(*[[st[k] for st in sts] for k in names], indices.to(torch.int64).contiguous())
             for k, column in zip(names, new):
                 for st, t in zip(sts, column):
                     st[k] = t

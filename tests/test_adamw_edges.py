@@ -490,6 +490,26 @@ def test_captured_steps_of_a_model(moments):
     assert fresh.steps == 1 and float(x[0]) == 4
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("moments", [32, 8])
+def test_rows_selected_by_32_bit_indices(moments):
+    """select_state takes what FusedAdam's takes: indices of 32 bits, and strided ones."""
+    import gsx  # noqa: F401
+    from gsx import optim
+    from tests.test_adamw import splat_model
+    out = []
+    index = torch.arange(210, -1, -1)
+    for form in (index.cuda(), index.int().cuda(), torch.stack([index, index], 1).cuda()[:, 0]):
+        opt = optim.FusedAdamW.for_splat_data(splat_model(211, 16, "cuda"), moments=moments)
+        for i, p in enumerate(opt.model.params()):
+            p.grad = torch.randn(p.shape, generator=torch.Generator().manual_seed(i)).cuda()
+        opt.step(2000)
+        opt.select_state(form)
+        out.append([t.cpu() for n in ("means", "sh0", "opacity") for t in opt.moment_values(n)])
+    for other in out[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(out[0], other))
+
+
 # ---- over ranks --------------------------------------------------------------------------------------------------------------------------------------------
 def _plain_adamw(params, exp_avgs, exp_avg_sqs, grads, lrs, weight_decays, beta1, beta2, eps, steps, control=None, splits=()):
     """ops.adamw_step_multi in torch operations of float32 on the CPU, value by value (so that a block of rows has the bits of the whole)."""
