@@ -353,8 +353,9 @@ GSX_DEV void select_pieces(const SelectRec& r, const int64_t* __restrict__ index
     }
 }
 
-// What bounds it: rows at random places of memory that comes in lines of 128 bytes.  1 M splats by a random order (122 MB of codes) miss the L2s 8.5 M times, a gigabyte, in
-// 171 us: rows of 48 bytes 85 of them, one to four bytes, of which every L2 fetches every line, the rest.  In an order near the old one, as a growth step's is: 81 us.
+// What bounds it, 1 M splats by a random order (122 MB of codes), 171 us: rows of 48 bytes (85 of them) the 128-byte lines that they lie in, 4.6 M misses at 6.9 TB/s; rows of
+// one to four bytes (92) the requests, one for every row and moment and one for its scale, 15 M (fewer misses there took the same time).  In an order near the old one, as a growth
+// step's is: 80 us.  100 k splats: 20 us, 16 in the near order: a round and a half of workgroups that wait for record, index and codes in turn.
 template <uint32_t L> __global__ __launch_bounds__(256, 8) void select_rows_kernel(SelectList<L> a) {
     __shared__ __align__(16) float lds[2][kSelect];
     walk(a.c, [&](const SelectRec& r, uint32_t chunk, uint32_t stop) {
